@@ -15,8 +15,10 @@ CSRC = os.path.join(HERE, 'csrc')
 OBJ = os.path.join(CSRC, 'build')
 LIB = os.path.join(HERE, 'librdfc_hip.so')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
+# -packed-fp32-ops: hipcc makes packed f32 instructions of ordinary float code by itself, and some of their forms have given wrong
+# results on gfx950 now and then (hipcc's host pass does not know the feature and says so: harmless)
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fno-gpu-rdc', '-Wno-unused-value',
-         '-Wno-pass-failed']
+         '-Wno-pass-failed', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def source_hash():
@@ -68,11 +70,16 @@ def _hash_object(force):
 
 def build(force=False, verbose=True):
     os.makedirs(OBJ, exist_ok=True)
+    stamp, line = os.path.join(OBJ, 'flags.txt'), ' '.join([HIPCC] + FLAGS) + '\n'
+    if not os.path.exists(stamp) or open(stamp).read() != line:          # objects of other flags are stale
+        force = True
     hdr = _deps_mtime()
     with ThreadPoolExecutor(max_workers=min(6, os.cpu_count() or 2)) as ex:
         res = list(ex.map(lambda s: _compile(s, hdr, force), _sources()))
     res.append(_hash_object(force))
     objs = [o for o, _ in res]
+    with open(stamp, 'w') as f:
+        f.write(line)
     if force or any(ch for _, ch in res) or not os.path.exists(LIB):
         subprocess.check_call([HIPCC, '--offload-arch=gfx950', '-shared', '-fPIC', '-o', LIB] + objs)
         if verbose:

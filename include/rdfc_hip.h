@@ -538,6 +538,58 @@ int rdfc_combine_scalars_backward(int n, const float *weights, float post, const
  * pairwise adds: encoder features feeding the next stage and a skip connection, rdf_generator.py:286-398). */
 int rdfc_sum_maps(int n, const void *const *srcs, const int *lds, void *dst, int P, int C, int ld_dst, int dtype, void *stream);
 
+/* ------------------------------------------------------------------------------
+ * Operators of transformer blocks on pixel-major maps (a pixel is a token).  None of them has a counterpart upstream.
+ * ------------------------------------------------------------------------------ */
+/* y[e] = keep(e) ? x[e] / (1 - threshold / 65536) : 0 over a map of P pixels and C channels; e: the element's index in the dense
+ * order.  keep(e): the 16-bit half e % 8 (low half of a word first) of the four words of Philox4x32-10 with counter (e / 8, offset) and
+ * key seed is not below `threshold` (0 .. 65536).  key: device memory {seed, offset} read in place of the two arguments, or NULL.
+ * The backward pass is the same call on the cotangent.  Nothing is stored.  y may be x. */
+int rdfc_dropout(const void *x, void *y, int64_t P, int C, int ldx, int ldy, int dtype, int threshold, uint64_t seed, uint64_t offset,
+                 const uint64_t *key, void *stream);
+/* one draw of a generator state in device memory: key = {state[0], state[1]}, state[1] += 1 (both: two uint64) */
+int rdfc_dropout_draw(uint64_t *state, uint64_t *key, void *stream);
+
+/* u = N_post(h) (post = 0: h);  y = x + scale[c] * gate[sample][c] * dropout(u);  n = N_pre(y) (pre = 0: not computed).
+ * N: RMS norm v * rsqrt(mean(v^2) + eps) * w (+ b), or layer norm (layer = 1) over the C channels of a pixel.  Dropout as in rdfc_dropout
+ * (threshold 0: none) on h's dense element index.  n is computed from y before its rounding to the map's type. */
+typedef struct rdfc_norm_residual_desc {
+    int64_t rows;                /* pixels per sample                                                    */
+    uint64_t seed, offset;
+    int32_t samples, C;          /* C <= 8192                                                            */
+    int32_t ldx, ldh, dtype;
+    int32_t layer, post, pre, threshold;
+    float eps;
+} rdfc_norm_residual_desc;
+/* x, h: maps of samples * rows pixels; gate f32 [samples][C], scale and the norms' parameters f32 [C], each may be NULL (1, or 0 for the
+ * biases).  y, n: dense [samples * rows][C].  h = NULL (with pre, without gate and scale): n = N_pre(x), y unused.
+ * stats: f32 [samples * rows][4] (16-byte aligned) for the backward pass, or NULL. */
+int rdfc_norm_residual(const rdfc_norm_residual_desc *d, const void *x, const void *h, const float *gate, const float *scale, const float *post_w,
+                       const float *post_b, const float *pre_w, const float *pre_b, const uint64_t *key, void *y, void *n, float *stats, void *stream);
+/* floats of scratch that the backward pass needs (gated: a gate is given) */
+size_t rdfc_norm_residual_scratch_floats(const rdfc_norm_residual_desc *d, int gated);
+/* dy, dn: cotangents of y and n (either may be NULL: zero).  dx, dh dense [samples * rows][C] (dh NULL with h); the parameter gradients
+ * f32, each may be NULL; scratch may be NULL if all of them are.  Column sums have a fixed order: the same bits every run. */
+int rdfc_norm_residual_backward(const rdfc_norm_residual_desc *d, const void *x, const void *h, const float *gate, const float *scale,
+                                const float *post_w, const float *post_b, const float *pre_w, const uint64_t *key, const float *stats,
+                                const void *dy, int lddy, const void *dn, int lddn, void *dx, void *dh, float *scratch, float *d_gate, float *d_scale,
+                                float *d_post_w, float *d_post_b, float *d_pre_w, float *d_pre_b, void *stream);
+
+/* z = act(x Wg^T + bg) * (x Wu^T + bu): x [M][K] (ldx), Wg, Wu [F][K] (ldwg, ldwu) of the map's type, bg, bu f32 [F] or both NULL, z dense [M][F].
+ * act: RDFC_ACT_RELU, RDFC_ACT_SIGMOID, RDFC_GATE_SILU or RDFC_GATE_GELU (the exact one). */
+enum { RDFC_GATE_SILU = 16, RDFC_GATE_GELU = 17 };
+typedef struct rdfc_gated_desc {
+    int64_t M;
+    int32_t K, F, ldx, ldwg, ldwu, dtype, act;
+} rdfc_gated_desc;
+int rdfc_gated_linear(const rdfc_gated_desc *d, const void *x, const void *wg, const void *wu, const float *bg, const float *bu, void *z, void *stream);
+size_t rdfc_gated_linear_scratch_bytes(const rdfc_gated_desc *d);
+/* dz [M][F] (lddz) -> dx dense [M][K], dwg, dwu dense [F][K] (dw_dtype: RDFC_F32 or the map's type), dbg, dbu f32 [F]; each may be NULL.
+ * scratch: 256-byte aligned.  g and u are computed again; dg and du are rounded to the map's type for the two products, the bias gradients
+ * are summed before that.  Sums have a fixed order. */
+int rdfc_gated_linear_backward(const rdfc_gated_desc *d, const void *x, const void *wg, const void *wu, const float *bg, const float *bu, const void *dz,
+                               int lddz, void *scratch, void *dx, void *dwg, void *dwu, int dw_dtype, float *dbg, float *dbu, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,551 @@
+// norm_residual.hip -- the junction of a residual stream with a block's output, between two row norms:
+//
+//     u = N_post(h)                                      (or h)
+//     y = x + scale[c] * gate[n][c] * dropout(u)         the residual stream behind the block
+//     n = N_pre(y)                                       the next block's input
+//
+// N: RMS norm v * rsqrt(mean(v^2) + eps) * w or layer norm (v - mean(v)) * rsqrt(var(v) + eps) * w + b over the C channels of a pixel.
+// A pixel's channels stay in the registers of the LPR lanes that own it from the load to the last store, so a pass moves x, h, y and n
+// once (forward) or x, h, dy, dn, dx and dh once (backward): HBM is the bound.  The backward pass recomputes y from x and h (the
+// same bytes as reading a saved y) in f32, so neither y nor the dropout mask nor the normalised maps are kept -- four f32 statistics
+// per pixel are.
+//
+// Column sums (gradients of the four norm parameters, of scale and of gate) reduce to four sums per sample and channel:
+//     A = sum D t hhat,  B = sum D t   (t: cotangent of y, D: dropout factor, hhat: normalised h, or h itself without N_post)
+//     P = sum dn yhat,   Q = sum dn
+// S = w A + b B is then the common part of d gate = scale S and d scale = sum_n gate S.  Each lane adds its own channels over
+// its rows in f32, workgroups write one partial row each, and a second kernel adds those in a fixed order in f64: no atomics, the same
+// bits every run.
+#include "philox.h"
+
+namespace {
+
+constexpr int NT = 256;
+
+struct NRArgs {
+    const void *x, *h;
+    void *y, *n;
+    const void *dy, *dn;
+    void *dx, *dh;
+    int64_t rows;                    // per sample
+    int C, ldx, ldh, ldy, ldn, lddy, lddn;
+    const float *gate, *scale, *post_w, *post_b, *pre_w, *pre_b;
+    int layer, post, pre;
+    float eps;
+    DropArgs drop;
+    f32x4 *stats;                    // per row: mean and reciprocal deviation of h, of y
+    float *partial;
+    int64_t chunk;                   // rows per workgroup
+};
+
+// ---- sums over the LPR lanes that own a row ------------------------------------------------------------------------------
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <int LPR> __device__ __forceinline__ float lanes_sum(float v) {
+    v = dpp_add<0xB1>(v);                                        // quad_perm 1,0,3,2
+    v = dpp_add<0x4E>(v);                                        // quad_perm 2,3,0,1
+    v = dpp_add<0x141>(v);                                       // row_half_mirror: eight lanes
+    if constexpr (LPR >= 16) v = dpp_add<0x140>(v);              // row_mirror
+    if constexpr (LPR >= 32) v += __shfl_xor(v, 16, 64);
+    if constexpr (LPR >= 64) v += __shfl_xor(v, 32, 64);
+    return v;
+}
+// two sums at once.  LPR = 256: over the workgroup, through LDS (`buf`: two slots of 8 floats used in turn; every thread calls)
+template <int LPR> __device__ __forceinline__ void row_sum2(float &a, float &b, float (*buf)[8], int &turn) {
+    a = lanes_sum<LPR>(a);
+    b = lanes_sum<LPR>(b);
+    if constexpr (LPR > 64) {
+        float *s = buf[turn];
+        turn ^= 1;
+        if ((threadIdx.x & 63) == 0) {
+            s[threadIdx.x >> 6] = a;
+            s[4 + (threadIdx.x >> 6)] = b;
+        }
+        __syncthreads();                                         // (the other slot is not written again before the next barrier)
+        a = (s[0] + s[1]) + (s[2] + s[3]);
+        b = (s[4] + s[5]) + (s[6] + s[7]);
+    }
+}
+
+// ---- eight channels ------------------------------------------------------------------------------------------------------
+// ALIGNED: C is a multiple of 8 and every row 16-byte aligned
+template <typename T, bool ALIGNED> __device__ __forceinline__ void load8(float (&v)[8], const T *row, int c, int C) {
+    if constexpr (ALIGNED) {
+        if (c >= C) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.f;
+        } else if constexpr (sizeof(T) == 4) {
+            Vec16<T> a, b;
+            a.load(row + c);
+            b.load(row + c + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = a.get(i), v[4 + i] = b.get(i);
+        } else {
+            Vec16<T> a;
+            a.load(row + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = a.get(i);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < C ? Elem<T>::ld(row + c + i) : 0.f;
+    }
+}
+template <typename T, bool ALIGNED> __device__ __forceinline__ void store8(const float (&v)[8], T *row, int c, int C) {
+    if constexpr (ALIGNED) {
+        if (c >= C) return;
+        if constexpr (sizeof(T) == 4) {
+            Vec16<T> a, b;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a.set(i, v[i]), b.set(i, v[4 + i]);
+            a.store(row + c);
+            b.store(row + c + 4);
+        } else {
+            Vec16<T> a;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a.set(i, v[i]);
+            a.store(row + c);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i < C) Elem<T>::st(row + c + i, v[i]);
+    }
+}
+// a parameter vector (f32, any alignment); a null pointer stands for `none`.  0 beyond C: what the lanes behind the last channel hold must
+// not enter a sum
+__device__ __forceinline__ void load_par(float (&v)[8], const float *p, int c, int C, float none) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i >= C ? 0.f : p != nullptr ? p[c + i] : none;
+}
+
+template <typename T, int LPR, int VPL, bool ALIGNED>
+__global__ __launch_bounds__(NT) void norm_residual_kernel(NRArgs p) {
+    constexpr int RPB = NT / LPR;
+    __shared__ float buf[2][8];
+    int turn = 0;
+    const int li = threadIdx.x % LPR, C = p.C;
+    const float rC = 1.f / (float)C;
+    const unsigned long long seed = p.drop.key ? p.drop.key[0] : p.drop.seed, offset = p.drop.key ? p.drop.key[1] : p.drop.offset;
+    float f[VPL][8], pw[VPL][8], pb[VPL][8], qw[VPL][8], qb[VPL][8];
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+        const int c = (v * LPR + li) * 8;
+        float g[8];
+        load_par(f[v], p.scale, c, C, 1.f);
+        load_par(g, p.gate ? p.gate + (size_t)blockIdx.y * C : nullptr, c, C, 1.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[v][i] *= g[i];
+        load_par(pw[v], p.post_w, c, C, 1.f);
+        load_par(pb[v], p.post_b, c, C, 0.f);
+        load_par(qw[v], p.pre_w, c, C, 1.f);
+        load_par(qb[v], p.pre_b, c, C, 0.f);
+    }
+    const int64_t r0 = (int64_t)blockIdx.x * p.chunk, r1 = min(r0 + p.chunk, p.rows), base = (int64_t)blockIdx.y * p.rows;
+    // mean and reciprocal deviation of the row in a[][]; a[][] becomes the normalised row
+    auto normalise = [&](float (&a)[VPL][8], float &mean, float &rstd) {
+        mean = 0.f;
+        float s = 0.f, z = 0.f;
+        if (p.layer) {
+#pragma unroll
+            for (int v = 0; v < VPL; ++v)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s += a[v][i];
+            row_sum2<LPR>(s, z, buf, turn);
+            mean = s * rC;
+        }
+        s = z = 0.f;
+#pragma unroll
+        for (int v = 0; v < VPL; ++v)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                a[v][i] = (v * LPR + li) * 8 + i < C ? a[v][i] - mean : 0.f;
+                s = fmaf(a[v][i], a[v][i], s);
+            }
+        row_sum2<LPR>(s, z, buf, turn);
+        rstd = 1.f / sqrtf(s * rC + p.eps);
+#pragma unroll
+        for (int v = 0; v < VPL; ++v)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[v][i] *= rstd;
+    };
+    for (int64_t r = r0 + threadIdx.x / LPR; r < r1; r += RPB) {
+        const int64_t row = base + r;
+        float a[VPL][8], b[VPL][8];
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) load8<T, ALIGNED>(a[v], (const T *)p.x + row * p.ldx, (v * LPR + li) * 8, C);
+        f32x4 st = {0.f, 0.f, 0.f, 0.f};
+        if (p.h != nullptr) {
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) load8<T, ALIGNED>(b[v], (const T *)p.h + row * p.ldh, (v * LPR + li) * 8, C);
+            if (p.post) {
+                float m, s;
+                normalise(b, m, s);
+                st[0] = m;
+                st[1] = s;
+            }
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) {
+                const int c = (v * LPR + li) * 8;
+                if (p.post) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) b[v][i] = fmaf(b[v][i], pw[v][i], pb[v][i]);
+                }
+                if (p.drop.threshold != 0) {
+                    const unsigned keep = keep8((unsigned long long)row * C + c, p.drop.threshold, seed, offset);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) b[v][i] = keep >> i & 1 ? b[v][i] * p.drop.inv : 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a[v][i] = fmaf(f[v][i], b[v][i], a[v][i]);
+                store8<T, ALIGNED>(a[v], (T *)p.y + row * p.ldy, c, C);
+            }
+        }
+        if (p.pre) {
+            float m, s;
+            normalise(a, m, s);
+            st[2] = m;
+            st[3] = s;
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a[v][i] = fmaf(a[v][i], qw[v][i], qb[v][i]);
+                store8<T, ALIGNED>(a[v], (T *)p.n + row * p.ldn, (v * LPR + li) * 8, C);
+            }
+        }
+        if (p.stats != nullptr && li == 0) p.stats[row] = st;
+    }
+}
+
+template <typename T, int LPR, int VPL, bool ALIGNED>
+__global__ __launch_bounds__(NT) void norm_residual_bwd_kernel(NRArgs p) {
+    constexpr int RPB = NT / LPR;
+    __shared__ float buf[2][8];
+    __shared__ float red[RPB > 1 ? (RPB / 2) * LPR * VPL * 8 : 1];
+    int turn = 0;
+    const int li = threadIdx.x % LPR, grp = threadIdx.x / LPR, C = p.C;
+    const float rC = 1.f / (float)C;
+    const unsigned long long seed = p.drop.key ? p.drop.key[0] : p.drop.seed, offset = p.drop.key ? p.drop.key[1] : p.drop.offset;
+    float f[VPL][8], pw[VPL][8], pb[VPL][8], qw[VPL][8];
+    float sum[4][VPL][8];                                        // A, B, P, Q
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+        const int c = (v * LPR + li) * 8;
+        float g[8];
+        load_par(f[v], p.scale, c, C, 1.f);
+        load_par(g, p.gate ? p.gate + (size_t)blockIdx.y * C : nullptr, c, C, 1.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[v][i] *= g[i];
+        load_par(pw[v], p.post_w, c, C, 1.f);
+        load_par(pb[v], p.post_b, c, C, 0.f);
+        load_par(qw[v], p.pre_w, c, C, 1.f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[k][v][i] = 0.f;
+    }
+    const int64_t r0 = (int64_t)blockIdx.x * p.chunk, r1 = min(r0 + p.chunk, p.rows), base = (int64_t)blockIdx.y * p.rows;
+    // gradient through a row norm: g = cotangent of the normalised row (0 beyond C), hat = the normalised row
+    auto through = [&](float (&g)[VPL][8], const float (&hat)[VPL][8], float rstd) {
+        float s = 0.f, z = 0.f;
+#pragma unroll
+        for (int v = 0; v < VPL; ++v)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                s = fmaf(g[v][i], hat[v][i], s);
+                z += g[v][i];
+            }
+        row_sum2<LPR>(s, z, buf, turn);
+        s *= rC;
+        z = p.layer ? z * rC : 0.f;
+#pragma unroll
+        for (int v = 0; v < VPL; ++v)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) g[v][i] = rstd * (g[v][i] - fmaf(hat[v][i], s, z));
+    };
+    for (int64_t r = r0 + grp; r < r1; r += RPB) {
+        const int64_t row = base + r;
+        float a[VPL][8], hat[VPL][8], t[VPL][8];
+        unsigned keep[VPL];
+        const f32x4 st = p.stats[row];
+        // hat = normalised h (or h), a = y
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) {
+            const int c = (v * LPR + li) * 8;
+            load8<T, ALIGNED>(a[v], (const T *)p.x + row * p.ldx, c, C);
+            keep[v] = 0xff;
+            if (p.h != nullptr) {
+                load8<T, ALIGNED>(hat[v], (const T *)p.h + row * p.ldh, c, C);
+                if (p.drop.threshold != 0) keep[v] = keep8((unsigned long long)row * C + c, p.drop.threshold, seed, offset);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float u = hat[v][i];
+                    if (p.post) {
+                        hat[v][i] = c + i < C ? (hat[v][i] - st[0]) * st[1] : 0.f;
+                        u = fmaf(hat[v][i], pw[v][i], pb[v][i]);
+                    }
+                    a[v][i] = fmaf(f[v][i], keep[v] >> i & 1 ? u * p.drop.inv : 0.f, a[v][i]);
+                }
+            }
+        }
+        // t = cotangent of y
+        if (p.dn != nullptr) {
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) {
+                const int c = (v * LPR + li) * 8;
+                load8<T, ALIGNED>(t[v], (const T *)p.dn + row * p.lddn, c, C);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    a[v][i] = c + i < C ? (a[v][i] - st[2]) * st[3] : 0.f;
+                    sum[2][v][i] = fmaf(t[v][i], a[v][i], sum[2][v][i]);
+                    sum[3][v][i] += t[v][i];
+                    t[v][i] *= qw[v][i];
+                }
+            }
+            through(t, a, st[3]);
+        } else {
+#pragma unroll
+            for (int v = 0; v < VPL; ++v)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[v][i] = 0.f;
+        }
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) {
+            const int c = (v * LPR + li) * 8;
+            if (p.dy != nullptr) {
+                float d[8];
+                load8<T, ALIGNED>(d, (const T *)p.dy + row * p.lddy, c, C);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[v][i] += d[i];
+            }
+            store8<T, ALIGNED>(t[v], (T *)p.dx + row * C, c, C);
+        }
+        if (p.h == nullptr) continue;
+#pragma unroll
+        for (int v = 0; v < VPL; ++v)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float d = keep[v] >> i & 1 ? t[v][i] * p.drop.inv : 0.f;
+                sum[0][v][i] = fmaf(d, hat[v][i], sum[0][v][i]);
+                sum[1][v][i] += d;
+                t[v][i] = d * f[v][i] * pw[v][i];
+            }
+        if (p.post) through(t, hat, st[1]);
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) store8<T, ALIGNED>(t[v], (T *)p.dh + row * C, (v * LPR + li) * 8, C);
+    }
+    // the row groups' sums, halved until one is left, then one partial row per sum: partial[sample][chunk][4][C]
+    if (p.partial == nullptr) return;
+    float *out = p.partial + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 * C;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        for (int half = RPB / 2; half > 0; half >>= 1) {
+            __syncthreads();
+            if (grp >= half && grp < 2 * half) {
+#pragma unroll
+                for (int v = 0; v < VPL; ++v)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) red[((grp - half) * LPR + li) * (VPL * 8) + v * 8 + i] = sum[k][v][i];
+            }
+            __syncthreads();
+            if (grp < half) {
+#pragma unroll
+                for (int v = 0; v < VPL; ++v)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum[k][v][i] += red[(grp * LPR + li) * (VPL * 8) + v * 8 + i];
+            }
+        }
+        if (grp == 0) {
+#pragma unroll
+            for (int v = 0; v < VPL; ++v)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if ((v * LPR + li) * 8 + i < C) out[(size_t)k * C + (v * LPR + li) * 8 + i] = sum[k][v][i];
+        }
+    }
+}
+
+// ---- column sums: 16 channels x 16 chunk lanes per workgroup --------------------------------------------------------------------
+struct NRGrads {
+    float *gate, *scale, *post_w, *post_b, *pre_w, *pre_b;       // each may be null
+};
+__global__ __launch_bounds__(NT) void norm_residual_cols_kernel(NRArgs p, NRGrads o, int samples, int nchunk) {
+    __shared__ double red[16][4][17];
+    const int cl = threadIdx.x & 15, kl = threadIdx.x >> 4, C = p.C, c = blockIdx.x * 16 + cl;
+    double dscale = 0., dpw = 0., dpb = 0., dqw = 0., dqb = 0.;
+    for (int g = 0; g < samples; ++g) {
+        double s[4] = {0., 0., 0., 0.};
+        if (c < C)
+            for (int k = kl; k < nchunk; k += 16)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[j] += (double)p.partial[(((size_t)g * nchunk + k) * 4 + j) * C + c];
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) red[kl][j][cl] = s[j];
+        __syncthreads();
+        if (kl == 0 && c < C) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[j] = 0.;
+                for (int k = 0; k < 16; ++k) s[j] += red[k][j][cl];
+            }
+            const double sc = p.scale ? p.scale[c] : 1., gt = p.gate ? p.gate[(size_t)g * C + c] : 1.;
+            const double S = p.post ? (p.post_w ? p.post_w[c] : 1.) * s[0] + (p.post_b ? p.post_b[c] : 0.) * s[1] : s[0];
+            if (o.gate) o.gate[(size_t)g * C + c] = (float)(sc * S);
+            dscale += gt * S;
+            dpw += sc * gt * s[0];
+            dpb += sc * gt * s[1];
+            dqw += s[2];
+            dqb += s[3];
+        }
+    }
+    if (kl == 0 && c < C) {
+        if (o.scale) o.scale[c] = (float)dscale;
+        if (o.post_w) o.post_w[c] = (float)dpw;
+        if (o.post_b) o.post_b[c] = (float)dpb;
+        if (o.pre_w) o.pre_w[c] = (float)dqw;
+        if (o.pre_b) o.pre_b[c] = (float)dqb;
+    }
+}
+
+constexpr int MAXC = 8192;
+// lanes and vectors of eight channels per lane: the fewest lanes that hold a row
+template <typename F> void with_layout(int C, F &&f) {
+    const int nv = (C + 7) / 8;
+    if (nv <= 8) f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
+    else if (nv <= 16) f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
+    else if (nv <= 32) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
+    else if (nv <= 64) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+    else if (nv <= 128) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+    else if (nv <= 256) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
+    else if (nv <= 512) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    else f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+}
+int lanes_of(int C) {
+    int l = 0;
+    with_layout(C, [&](auto lpr, auto) { l = decltype(lpr)::value; });
+    return l;
+}
+// rows per workgroup: about 1024 workgroups, each row group at least four rows (the backward kernel leaves 4 C sums per workgroup)
+int64_t chunk_of(int64_t rows, int samples, int C) {
+    const int64_t rpb = NT / lanes_of(C), total = rows * samples;
+    int64_t per = (total + 1023) / 1024;
+    per = per < 4 * rpb ? 4 * rpb : per;
+    per = (per + rpb - 1) / rpb * rpb;
+    while ((rows + per - 1) / per >= (1 << 20)) per *= 2;
+    return per;
+}
+bool row_aligned(const void *p, int ld, int dtype) { return (reinterpret_cast<size_t>(p) & 15) == 0 && ld % rdfc_vec(dtype) == 0; }
+
+}  // namespace
+
+static int nr_check(const rdfc_norm_residual_desc *d, const char *name) {
+    RDFC_REQUIRE(d != nullptr, "%s: null descriptor", name);
+    RDFC_REQUIRE(rdfc_dtype_ok(d->dtype), "%s: unsupported dtype %d", name, d->dtype);
+    RDFC_REQUIRE(d->samples >= 0 && d->samples <= 65535 && d->rows >= 0, "%s: bad sizes samples=%d rows=%lld", name, d->samples, (long long)d->rows);
+    RDFC_REQUIRE(d->C > 0 && d->C <= MAXC, "%s: C = %d is not in [1, %d]", name, d->C, MAXC);
+    RDFC_REQUIRE(d->ldx >= d->C && d->ldh >= d->C, "%s: ld smaller than C", name);
+    RDFC_REQUIRE(d->threshold >= 0 && d->threshold <= 65536, "%s: threshold %d is not in [0, 65536]", name, d->threshold);
+    return 0;
+}
+static NRArgs nr_args(const rdfc_norm_residual_desc *d, const void *x, const void *h, const float *gate, const float *scale, const float *post_w,
+                      const float *post_b, const float *pre_w, const float *pre_b, const uint64_t *key) {
+    NRArgs p = {};
+    p.x = x;
+    p.h = h;
+    p.rows = d->rows;
+    p.C = d->C;
+    p.ldx = d->ldx;
+    p.ldh = d->ldh;
+    p.gate = gate;
+    p.scale = scale;
+    p.post_w = post_w;
+    p.post_b = post_b;
+    p.pre_w = pre_w;
+    p.pre_b = pre_b;
+    p.layer = d->layer;
+    p.post = d->post && h != nullptr;
+    p.pre = d->pre;
+    p.eps = d->eps;
+    drop_args(p.drop, d->threshold, d->seed, d->offset, key);
+    return p;
+}
+
+extern "C" int rdfc_norm_residual(const rdfc_norm_residual_desc *d, const void *x, const void *h, const float *gate, const float *scale,
+                                  const float *post_w, const float *post_b, const float *pre_w, const float *pre_b, const uint64_t *key, void *y,
+                                  void *n, float *stats, void *stream) {
+    if (nr_check(d, "rdfc_norm_residual")) return 1;
+    if (d->samples == 0 || d->rows == 0) return 0;
+    RDFC_REQUIRE(x && (h ? y != nullptr : (d->pre && !gate && !scale)) && (!d->pre || n), "rdfc_norm_residual: null map");
+    NRArgs p = nr_args(d, x, h, gate, scale, post_w, post_b, pre_w, pre_b, key);
+    p.y = y;
+    p.n = n;
+    p.ldy = p.ldn = d->C;
+    p.stats = reinterpret_cast<f32x4 *>(stats);
+    // (without a gate the samples are one run of rows)
+    const int samples = gate ? d->samples : 1;
+    p.rows = gate ? d->rows : d->rows * d->samples;
+    p.chunk = chunk_of(p.rows, samples, d->C);
+    const dim3 grid((unsigned)((p.rows + p.chunk - 1) / p.chunk), samples);
+    const bool al = row_aligned(x, d->ldx, d->dtype) && row_aligned(h, d->ldh, d->dtype) && row_aligned(y, d->C, d->dtype) && row_aligned(n, d->C, d->dtype) && d->C % 8 == 0;
+    with_layout(d->C, [&](auto lpr, auto vpl) {
+        constexpr int L = decltype(lpr)::value, V = decltype(vpl)::value;
+        RDFC_DISPATCH(d->dtype, if (al) norm_residual_kernel<T, L, V, true><<<grid, NT, 0, (hipStream_t)stream>>>(p);
+                      else norm_residual_kernel<T, L, V, false><<<grid, NT, 0, (hipStream_t)stream>>>(p));
+    });
+    RDFC_LAUNCH_CHECK("rdfc_norm_residual");
+    return 0;
+}
+
+extern "C" size_t rdfc_norm_residual_scratch_floats(const rdfc_norm_residual_desc *d, int gated) {
+    if (nr_check(d, "rdfc_norm_residual_scratch_floats") || d->samples == 0 || d->rows == 0) return 0;
+    const int samples = gated ? d->samples : 1;
+    const int64_t rows = gated ? d->rows : d->rows * d->samples, chunk = chunk_of(rows, samples, d->C);
+    return (size_t)samples * (size_t)((rows + chunk - 1) / chunk) * 4 * d->C;
+}
+
+extern "C" int rdfc_norm_residual_backward(const rdfc_norm_residual_desc *d, const void *x, const void *h, const float *gate, const float *scale,
+                                           const float *post_w, const float *post_b, const float *pre_w, const uint64_t *key, const float *stats,
+                                           const void *dy, int lddy, const void *dn, int lddn, void *dx, void *dh, float *scratch, float *d_gate,
+                                           float *d_scale, float *d_post_w, float *d_post_b, float *d_pre_w, float *d_pre_b, void *stream) {
+    if (nr_check(d, "rdfc_norm_residual_backward")) return 1;
+    RDFC_REQUIRE(!dy || lddy >= d->C, "rdfc_norm_residual_backward: lddy smaller than C");
+    RDFC_REQUIRE(!dn || lddn >= d->C, "rdfc_norm_residual_backward: lddn smaller than C");
+    const bool cols = d_gate || d_scale || d_post_w || d_post_b || d_pre_w || d_pre_b;
+    const bool empty = d->samples == 0 || d->rows == 0;
+    if (empty && !cols) return 0;
+    if (!empty) RDFC_REQUIRE(x && dx && (!h || dh) && stats && (!dn || d->pre) && (!cols || scratch), "rdfc_norm_residual_backward: null pointer");
+    RDFC_REQUIRE(!d_gate || gate, "rdfc_norm_residual_backward: gradient of a gate that is not there");
+    NRArgs p = nr_args(d, x, h, gate, scale, post_w, post_b, pre_w, nullptr, key);
+    p.dy = dy;
+    p.dn = dn;
+    p.lddy = lddy;
+    p.lddn = lddn;
+    p.dx = dx;
+    p.dh = dh;
+    p.stats = reinterpret_cast<f32x4 *>(const_cast<float *>(stats));
+    p.partial = cols ? scratch : nullptr;
+    const int samples = gate ? d->samples : 1;
+    int nchunk = 0;
+    if (!empty) {
+        p.rows = gate ? d->rows : d->rows * d->samples;
+        p.chunk = chunk_of(p.rows, samples, d->C);
+        nchunk = (int)((p.rows + p.chunk - 1) / p.chunk);
+        const dim3 grid((unsigned)nchunk, samples);
+        const bool al = row_aligned(x, d->ldx, d->dtype) && row_aligned(h, d->ldh, d->dtype) && row_aligned(dy, lddy, d->dtype) &&
+                        row_aligned(dn, lddn, d->dtype) && row_aligned(dx, d->C, d->dtype) && row_aligned(dh, d->C, d->dtype) && d->C % 8 == 0;
+        with_layout(d->C, [&](auto lpr, auto vpl) {
+            constexpr int L = decltype(lpr)::value, V = decltype(vpl)::value;
+            RDFC_DISPATCH(d->dtype, if (al) norm_residual_bwd_kernel<T, L, V, true><<<grid, NT, 0, (hipStream_t)stream>>>(p);
+                          else norm_residual_bwd_kernel<T, L, V, false><<<grid, NT, 0, (hipStream_t)stream>>>(p));
+        });
+        RDFC_LAUNCH_CHECK("rdfc_norm_residual_backward");
+    }
+    if (cols) {
+        const NRGrads o = {d_gate, d_scale, d_post_w, d_post_b, d_pre_w, d_pre_b};
+        norm_residual_cols_kernel<<<cdiv(d->C, 16), NT, 0, (hipStream_t)stream>>>(p, o, samples, nchunk);
+        RDFC_LAUNCH_CHECK("rdfc_norm_residual_backward (columns)");
+    }
+    return 0;
+}

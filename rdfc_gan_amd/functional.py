@@ -9,6 +9,9 @@ Blocks
   conv_block   conv | conv-transpose  [+bias] [+BatchNorm | InstanceNorm] [+residual] [+act]
   wadain       W-AdaIN fusion (per-pixel style affine of an instance-normalised map)
   crop_cat     upstream's `_concat` (crop trailing rows/cols, concatenate channels)
+  dropout      elementwise dropout from a counter-based generator, no stored mask
+  norm_residual, row_norm   norm behind a block + gate + scale + dropout + residual + norm before the next block
+  gated_linear act(x Wg^T + bg) * (x Wu^T + bu)
   reflect_pad, to_pm / to_nchw, fusion_head
 """
 import math
@@ -1019,3 +1022,232 @@ class _NormalLosses(torch.autograd.Function):
 def normal_losses(normal, gt_normal, norm_mask, logits_nchw, label_wall, label_floor, label_ceiling):
     return _NormalLosses.apply(normal, gt_normal, norm_mask, logits_nchw.detach() if logits_nchw is not None else None,
                                (label_wall, label_floor, label_ceiling))
+
+
+# ---- operators of transformer blocks on pixel-major maps (a pixel is a token) ----------------------------------------------------
+class DropoutState:
+    """Generator state {seed, counter} in device memory.  Every draw copies it into a key of its own and advances the counter, on the
+    current stream: a captured HIP graph draws new masks at every replay, and a backward pass reads its own forward's key."""
+
+    def __init__(self, seed=None, device='cuda'):
+        seed = torch.initial_seed() if seed is None else int(seed)
+        self.state = torch.tensor([_signed64(seed), 0], dtype=torch.int64, device=device)
+
+    def draw(self):
+        return hip.dropout_draw(self.state)
+
+
+def _signed64(v):
+    v &= 0xffffffffffffffff
+    return v - (1 << 64) if v >> 63 else v
+
+
+def _drop_rng(p, training, rng, x):
+    """checks what is drawn for the map x -> (threshold of 65536, seed, offset, device key | None)"""
+    device = x.device
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f'dropout probability {p} is not in [0, 1]')
+    threshold = int(p * 65536 + 0.5) if training else 0
+    if threshold == 0:
+        return 0, 0, 0, None
+    if isinstance(rng, DropoutState):
+        if rng.state.device != device:                # (before the draw: a refused call advances nothing)
+            raise ValueError(f'the DropoutState is on {rng.state.device}, the map on {device}')
+        _check_device(x, 'dropout')
+        return threshold, 0, 0, rng.draw()
+    if rng is not None:
+        seed, offset = (int(v) for v in rng)
+        if not (0 <= seed < 1 << 64 and 0 <= offset < 1 << 64):
+            raise ValueError(f'seed and offset are unsigned 64-bit numbers, got {rng}')
+        _check_device(x, 'dropout')
+        return threshold, seed, offset, None
+    _check_device(x, 'dropout')
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError('dropout inside a HIP graph: pass rng=DropoutState(...) (torch\'s generator would give every replay the same mask)')
+    gen = torch.cuda.default_generators[device.index]
+    at = gen.get_offset()
+    gen.set_offset(at + 4)
+    return threshold, gen.initial_seed() & 0xffffffffffffffff, 1 << 63 | at, None        # (bit 63: apart from the counters of torch's own kernels)
+
+
+def _check_map(t, what, like=None):
+    if not isinstance(t, torch.Tensor) or t.dim() != 4:
+        raise ValueError(f'{what}: a pixel-major map [N, H, W, C] is needed')
+    if t.shape[3] < 1:
+        raise ValueError(f'{what}: no channels')
+    if like is None:
+        hip.dt(t)
+    elif t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f'{what}: {t.dtype} on {t.device} beside a map of {like.dtype} on {like.device}')
+
+
+def _check_device(t, what):
+    if not t.is_cuda:
+        raise ValueError(f'{what}: the HIP kernels need device tensors, this one is on {t.device}')
+
+
+def _check_param(t, what, shape, device):
+    """a parameter vector: f32 (cast where it is not), dense"""
+    if t is None:
+        return None
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f'{what}: shape {tuple(t.shape)}, expected {tuple(shape)}')
+    if t.device != device or not t.is_floating_point():
+        raise ValueError(f'{what}: {t.dtype} on {t.device}, expected a floating type on {device}')
+    return t.float().contiguous()
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, threshold, seed, offset, key):
+        ctx.args = threshold, seed, offset, key
+        return hip.dropout(hip.as_pm(x), threshold, seed, offset, key)
+
+    @staticmethod
+    def backward(ctx, dy):
+        return _Dropout.apply(dy, *ctx.args), None, None, None, None
+
+
+def dropout(x, p, training=True, rng=None):
+    """nn.Dropout on a pixel-major map: an element is zeroed with probability T / 65536, T = round(65536 p), the others are scaled by
+    1 / (1 - T / 65536).  The mask is a function of (seed, offset, element) -- Philox4x32-10, csrc/philox.h -- and is drawn again by the
+    backward pass, not stored.  rng: None (torch's generator of the device: its seed, and an offset that every call advances by 4), a pair
+    (seed, offset), or a DropoutState (needed inside a captured graph)."""
+    _check_map(x, 'dropout')
+    threshold, seed, offset, key = _drop_rng(p, training, rng, x)
+    return _Dropout.apply(x, threshold, seed, offset, key) if threshold else x
+
+
+class _NormResidual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, h, gate, scale, post_w, post_b, pre_w, pre_b, has_post, has_pre, layer, eps, drop):
+        x = hip.as_pm(x)
+        h = hip.as_pm(h) if h is not None else None
+        post, pre = (post_w, post_b) if has_post else None, (pre_w, pre_b) if has_pre else None
+        d, y, n, stats = hip.norm_residual(x, h, gate, scale, post, pre, layer, eps, *drop, want_stats=any(ctx.needs_input_grad))
+        ctx.save_for_backward(x, h, gate, scale, post_w, post_b, pre_w, stats, drop[3])
+        ctx.meta = d, has_post, has_pre
+        ctx.set_materialize_grads(False)
+        return y, n
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dn):
+        x, h, gate, scale, post_w, post_b, pre_w, stats, key = ctx.saved_tensors
+        d, has_post, has_pre = ctx.meta
+        if dy is None and dn is None:
+            return (None,) * 13
+        dy, dn = (None if g is None else hip.as_pm(g if g.dtype == x.dtype else g.to(x.dtype)) for g in (dy, dn))
+        grads = hip.norm_residual_backward(d, x, h, gate, scale, (post_w, post_b) if has_post else None, (pre_w, None) if has_pre else None, key, stats,
+                                           dy, dn, ctx.needs_input_grad[2:8])
+        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None, None, None)
+
+
+def _norm_params(wb, what, C, device):
+    """(weight | None, bias | None), or a weight alone"""
+    if wb is None:
+        return False, None, None
+    w, b = wb if isinstance(wb, (tuple, list)) else (wb, None)
+    return True, _check_param(w, f'{what} weight', (C,), device), _check_param(b, f'{what} bias', (C,), device)
+
+
+def _norm_kind(norm, eps):
+    if norm not in ('rms', 'layer'):
+        raise ValueError(f"norm is 'rms' or 'layer', got {norm!r}")
+    if not eps >= 0.0:
+        raise ValueError(f'eps = {eps} is negative')
+    return norm == 'layer'
+
+
+def norm_residual(x, h, *, gate=None, scale=None, post=None, pre=None, norm='rms', eps=1e-5, p=0.0, training=True, rng=None):
+    """The junction of a residual stream x with a block's output h, one kernel:
+
+        u = N_post(h)                                 post: (weight [C] | None, bias [C] | None); None: u = h
+        y = x + scale * gate * dropout(u, p)          scale [C], gate [N, C] (or [N, 1, 1, C]); None: 1
+        n = N_pre(y)                                  pre: like post; None: n is None
+
+    -> (y, n).  N is an RMS or a layer norm over the channels of a pixel; its statistics, and y on its way into n, are f32.  C <= 8192.
+    The parameters are f32; gate and scale may be activations (they are cast and get gradients like any input)."""
+    _check_map(x, 'norm_residual')
+    _check_map(h, 'norm_residual: h', x)
+    if h.shape != x.shape:
+        raise ValueError(f'norm_residual: h {tuple(h.shape)} beside x {tuple(x.shape)}')
+    layer = _norm_kind(norm, eps)
+    N, _, _, C = x.shape
+    if C > 8192:
+        raise ValueError(f'norm_residual: {C} channels, at most 8192')
+    if N > 65535 and gate is not None:
+        raise ValueError(f'norm_residual: a gate for {N} samples, at most 65535')
+    if gate is not None and gate.dim() == 4 and gate.shape[1:3] == (1, 1):
+        gate = gate.flatten(1)
+    gate, scale = _check_param(gate, 'gate', (N, C), x.device), _check_param(scale, 'scale', (C,), x.device)
+    has_post, post_w, post_b = _norm_params(post, 'post', C, x.device)
+    has_pre, pre_w, pre_b = _norm_params(pre, 'pre', C, x.device)
+    drop = _drop_rng(p, training, rng, x)
+    _check_device(x, 'norm_residual')
+    return _NormResidual.apply(x, h, gate, scale, post_w, post_b, pre_w, pre_b, has_post, has_pre, layer, float(eps), drop)
+
+
+def row_norm(x, weight=None, bias=None, norm='rms', eps=1e-5):
+    """RMS or layer norm over the channels of every pixel: norm_residual's N_pre alone (in front of the first block of a residual stream)"""
+    _check_map(x, 'row_norm')
+    layer = _norm_kind(norm, eps)
+    C = x.shape[3]
+    if C > 8192:
+        raise ValueError(f'row_norm: {C} channels, at most 8192')
+    _, w, b = _norm_params((weight, bias), 'row_norm', C, x.device)
+    _check_device(x, 'row_norm')
+    return _NormResidual.apply(x, None, None, None, None, None, w, b, False, True, layer, float(eps), (0, 0, 0, None))[1]
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, wg, wu, bg, bu, act):
+        x = hip.as_pm(x)
+        ctx.dw_dtype = wg.dtype
+        wg, wu = (_weight_rows(w, x.dtype) for w in (wg, wu))
+        d, z = hip.gated_linear(x, wg, wu, bg, bu, act)
+        ctx.save_for_backward(x, wg, wu, bg, bu)
+        ctx.desc = d
+        return z
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dz):
+        x, wg, wu, bg, bu = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dz = hip.as_pm(dz if dz.dtype == x.dtype else dz.to(x.dtype))
+        grads = hip.gated_linear_backward(ctx.desc, x, wg, wu, bg, bu, dz, need[0], ctx.dw_dtype if need[1] or need[2] else None, need[3] or need[4])
+        return (*(g if n else None for g, n in zip(grads, need)), None)
+
+
+def _weight_rows(w, dtype):
+    """weights [F, K] in the map's type with dense rows"""
+    w = w.to(dtype)
+    return w if w.stride(1) == 1 and w.stride(0) >= w.shape[1] and w.stride(0) < 2 ** 31 else w.contiguous()
+
+
+def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act='silu'):
+    """z = act(x w_gate^T + b_gate) * (x w_up^T + b_up) on a pixel-major map x [N, H, W, K] -> [N, H, W, F]: both projections, the activation
+    and the product in one kernel.  w_gate, w_up [F, K] (or 1x1 convolution weights [F, K, 1, 1]) in the map's type, or f32 masters beside a
+    16-bit map (cast in the call; their gradients are then f32); b_gate, b_up f32 [F], both or neither.  act: 'silu', 'gelu' (exact),
+    'sigmoid' or 'relu'.  The backward pass computes both projections again; in 16-bit maps their cotangents are rounded to the map's
+    type before the products with the weights and with x, as every block here stores its cotangents."""
+    _check_map(x, 'gated_linear')
+    if act not in hip.GATE_ACT:
+        raise ValueError(f'act is one of {sorted(hip.GATE_ACT)}, got {act!r}')
+    w_gate, w_up = (w.flatten(1) if w.dim() == 4 and w.shape[2:] == (1, 1) else w for w in (w_gate, w_up))
+    K = x.shape[3]
+    if w_gate.dim() != 2 or w_gate.shape != w_up.shape or w_gate.shape[1] != K or w_gate.shape[0] < 1:
+        raise ValueError(f'gated_linear: weights {tuple(w_gate.shape)} and {tuple(w_up.shape)} for {K} channels')
+    F = w_gate.shape[0]
+    if F > 1 << 20 or K > 1 << 20:
+        raise ValueError(f'gated_linear: weights {tuple(w_gate.shape)}, at most 2^20 rows and columns')
+    for w in (w_gate, w_up):
+        if w.dtype not in (x.dtype, torch.float32) or w.dtype != w_gate.dtype or w.device != x.device:
+            raise ValueError(f'gated_linear: weights of {w_gate.dtype} / {w_up.dtype} on {w.device} beside a map of {x.dtype} on {x.device}')
+    if (b_gate is None) != (b_up is None):
+        raise ValueError('gated_linear: one bias without the other')
+    b_gate, b_up = _check_param(b_gate, 'b_gate', (F,), x.device), _check_param(b_up, 'b_up', (F,), x.device)
+    _check_device(x, 'gated_linear')
+    return _GatedLinear.apply(x, w_gate, w_up, b_gate, b_up, act)

@@ -16,7 +16,7 @@ import torch
 import torch.nn as nn
 
 from . import functional as Fh
-from .layers import ConvSeq, conv_bn_relu, convt_bn_relu, resnet_stage, run_conv
+from .layers import ConvSeq, Dropout, conv_bn_relu, convt_bn_relu, resnet_stage, run_conv
 from .nlspn import NLSPNRefineModule
 
 _RESNET_LAYERS = {'resnet18': (2, 2, 2, 2), 'resnet34': (3, 4, 6, 3)}
@@ -254,19 +254,22 @@ class RDFGenerator(nn.Module):
 class ResnetBlock(nn.Module):
     def __init__(self, dim, padding_type, norm_layer, use_dropout, use_bias):
         super().__init__()
-        if padding_type != 'reflect' or use_dropout:
-            raise NotImplementedError('HIP path covers reflect padding without dropout (the shipped configuration)')
+        if padding_type != 'reflect':
+            raise NotImplementedError('HIP path covers reflect padding (the shipped configuration)')
         self.conv_block = nn.Sequential(
             nn.ReflectionPad2d(1), nn.Conv2d(dim, dim, kernel_size=3, padding=0, bias=use_bias), norm_layer(dim),
-            nn.LeakyReLU(negative_slope=0.01, inplace=True),
+            nn.LeakyReLU(negative_slope=0.01, inplace=True), *([Dropout(0.5)] if use_dropout else []),
             nn.ReflectionPad2d(1), nn.Conv2d(dim, dim, kernel_size=3, padding=0, bias=use_bias), norm_layer(dim))
+        self.use_dropout = use_dropout
 
     def forward(self, x):
         cb = self.conv_block
         # ReflectionPad2d(1) + conv as ONE block: the pad is folded into the conv's loaders (functional.ConvSpec.reflect); the skip's
         # cotangent is added inside the pad's adjoint kernel in the backward
         y, xr = run_conv(x, cb[1], cb[2], cb[3], reflect=1, passthrough=True)
-        return run_conv(y, cb[5], cb[6], None, res=xr, reflect=1)             # out = x + conv_block(x)
+        if self.use_dropout:
+            y = cb[4](y)
+        return run_conv(y, cb[-2], cb[-1], None, res=xr, reflect=1)           # out = x + conv_block(x)
 
 
 class ResnetGenerator(nn.Module):

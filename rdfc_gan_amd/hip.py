@@ -52,6 +52,8 @@ def lib():
         _lib.rdfc_last_error.restype = C.c_char_p
         _lib.rdfc_last_kernel.restype = C.c_char_p
         _lib.rdfc_build_hash.restype = C.c_char_p
+        _lib.rdfc_norm_residual_scratch_floats.argtypes, _lib.rdfc_norm_residual_scratch_floats.restype = [C.c_void_p, C.c_int], C.c_size_t
+        _lib.rdfc_gated_linear_scratch_bytes.argtypes, _lib.rdfc_gated_linear_scratch_bytes.restype = [C.c_void_p], C.c_size_t
         _declare_argtypes(_lib)
     return _lib
 
@@ -1041,3 +1043,106 @@ def normal_losses_backward(normal, gt_normal, norm_mask, logits_nchw, label_wall
     _chk(lib().rdfc_normal_losses_backward(_p(normal), _p(gt), _p(m), _p(z), N, HW, Cc, ldz, label_wall, label_floor, label_ceiling,
                                            _p(out8), _p(grad4.contiguous().float()), _p(g), _st()), 'rdfc_normal_losses_backward')
     return g
+
+
+# --------------------------------------------------------------------------- transformer-block operators
+class NormResidualDesc(C.Structure):
+    _fields_ = [('rows', C.c_int64), ('seed', C.c_uint64), ('offset', C.c_uint64)] + \
+               [(n, C.c_int32) for n in ('samples', 'C', 'ldx', 'ldh', 'dtype', 'layer', 'post', 'pre', 'threshold')] + [('eps', C.c_float)]
+
+
+class GatedDesc(C.Structure):
+    _fields_ = [('M', C.c_int64)] + [(n, C.c_int32) for n in ('K', 'F', 'ldx', 'ldwg', 'ldwu', 'dtype', 'act')]
+
+
+GATE_ACT = dict(relu=1, sigmoid=4, silu=16, gelu=17)
+
+
+def _call(name, t, *args):
+    """one entry point on t's device and that device's current stream (whatever the current device is)"""
+    fn, dev = getattr(lib(), name), t.device.index
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc != 0:
+        _chk(rc, name)
+
+
+def as_pm(t):
+    """t itself where the kernels can read it through (pointer, ld), else a dense copy"""
+    if t.is_contiguous():
+        return t
+    return t if is_pm(t) and ld(t) < 2 ** 31 else t.contiguous()
+
+
+def dropout(x, threshold, seed, offset, key=None):
+    """keep mask of (seed, offset), or of `key` (device int64 [2]), applied to a pixel-major map"""
+    N, H, W, Cc = x.shape
+    y = torch.empty(N, H, W, Cc, dtype=x.dtype, device=x.device)
+    if y.numel():
+        _call('rdfc_dropout', x, _p(x), _p(y), N * H * W, Cc, ld(x), Cc, dt(x), threshold, seed, offset, _p(key))
+    return y
+
+
+def dropout_draw(state):
+    key = torch.empty(2, dtype=torch.int64, device=state.device)
+    _call('rdfc_dropout_draw', state, _p(state), _p(key))
+    return key
+
+
+def norm_residual(x, h, gate, scale, post, pre, layer, eps, threshold, seed, offset, key, want_stats):
+    """-> (descriptor, y, n, stats); post / pre: (weight | None, bias | None) or None"""
+    N, H, W, Cc = x.shape
+    samples = N if gate is not None else 1                   # (without a gate the samples are one run of rows)
+    d = NormResidualDesc(N * H * W // samples if samples else 0, seed, offset, samples, Cc, ld(x), ld(h) if h is not None else Cc, dt(x), int(layer), int(post is not None),
+                         int(pre is not None), threshold, eps)
+    y = torch.empty(N, H, W, Cc, dtype=x.dtype, device=x.device) if h is not None else None
+    n = torch.empty(N, H, W, Cc, dtype=x.dtype, device=x.device) if pre is not None else None
+    stats = torch.empty(N * H * W, 4, dtype=torch.float32, device=x.device) if want_stats else None
+    if x.numel():
+        pw, pb = post or (None, None)
+        qw, qb = pre or (None, None)
+        _call('rdfc_norm_residual', x, C.byref(d), _p(x), _p(h), _p(gate), _p(scale), _p(pw), _p(pb), _p(qw), _p(qb), _p(key), _p(y), _p(n), _p(stats))
+    return d, y, n, stats
+
+
+def norm_residual_backward(d, x, h, gate, scale, post, pre, key, stats, dy, dn, want):
+    """want: which of (gate, scale, post_w, post_b, pre_w, pre_b) need a gradient -> (dx, dh, those six)"""
+    N, H, W, Cc = x.shape
+    pw, pb = post or (None, None)
+    qw = pre[0] if pre else None
+    dx = torch.empty(N, H, W, Cc, dtype=x.dtype, device=x.device)
+    dh = torch.empty_like(dx) if h is not None else None
+    cols = [torch.empty((N, Cc) if i == 0 else (Cc,), dtype=torch.float32, device=x.device) if w else None for i, w in enumerate(want)]
+    scratch = None
+    if any(want):
+        scratch = torch.empty(lib().rdfc_norm_residual_scratch_floats(C.byref(d), int(gate is not None)), dtype=torch.float32, device=x.device)
+    _call('rdfc_norm_residual_backward', x, C.byref(d), _p(x), _p(h), _p(gate), _p(scale), _p(pw), _p(pb), _p(qw), _p(key), _p(stats), _p(dy),
+          ld(dy) if dy is not None else Cc, _p(dn), ld(dn) if dn is not None else Cc, _p(dx), _p(dh), _p(scratch), *map(_p, cols))
+    return (dx, dh, *cols)
+
+
+def gated_linear(x, wg, wu, bg, bu, act):
+    """-> (descriptor, z); x pixel-major, weights [F, K] rows of the map's type"""
+    N, H, W, K = x.shape
+    F = wg.shape[0]
+    d = GatedDesc(N * H * W, K, F, ld(x), wg.stride(0) if F > 1 else K, wu.stride(0) if F > 1 else K, dt(x), GATE_ACT[act])
+    z = torch.empty(N, H, W, F, dtype=x.dtype, device=x.device)
+    if z.numel():
+        _call('rdfc_gated_linear', x, C.byref(d), _p(x), _p(wg), _p(wu), _p(bg), _p(bu), _p(z))
+    return d, z
+
+
+def gated_linear_backward(d, x, wg, wu, bg, bu, dz, want_dx, dw_dtype, want_bias):
+    """dw_dtype: None (no weight gradients), f32 or the map's type -> (dx, dwg, dwu, dbg, dbu)"""
+    N, H, W, K = x.shape
+    F = wg.shape[0]
+    dx = torch.empty(N, H, W, K, dtype=x.dtype, device=x.device) if want_dx else None
+    dwg, dwu = (torch.empty(F, K, dtype=dw_dtype, device=x.device) for _ in range(2)) if dw_dtype is not None else (None, None)
+    dbg, dbu = (torch.empty(F, dtype=torch.float32, device=x.device) for _ in range(2)) if want_bias else (None, None)
+    scratch = torch.empty(lib().rdfc_gated_linear_scratch_bytes(C.byref(d)), dtype=torch.uint8, device=x.device)
+    _call('rdfc_gated_linear_backward', x, C.byref(d), _p(x), _p(wg), _p(wu), _p(bg), _p(bu), _p(dz), ld(dz), _p(scratch), _p(dx), _p(dwg), _p(dwu),
+          F32 if dw_dtype == torch.float32 else dt(x), _p(dbg), _p(dbu))
+    return dx, dwg, dwu, dbg, dbu

@@ -186,3 +186,68 @@ class BasicBlock(nn.Module):
 
 def resnet_stage(cin, cout, stride, blocks):
     return nn.Sequential(*[BasicBlock(cin if i == 0 else cout, cout, stride if i == 0 else 1) for i in range(blocks)])
+
+
+class Dropout(nn.Dropout):
+    """nn.Dropout on pixel-major maps (functional.dropout); rng: what that call takes, e.g. a functional.DropoutState"""
+    rng = None
+
+    def forward(self, x):
+        return Fh.dropout(x, self.p, self.training, self.rng)
+
+
+class RowNorm(nn.Module):
+    """RMS or layer norm over the channels of every pixel of a pixel-major map"""
+
+    def __init__(self, dim, norm='rms', eps=1e-5):
+        super().__init__()
+        self.norm, self.eps = norm, eps
+        self.weight = nn.Parameter(torch.ones(dim))
+        self.bias = nn.Parameter(torch.zeros(dim)) if norm == 'layer' else None
+
+    def forward(self, x):
+        return Fh.row_norm(x, self.weight, self.bias, self.norm, self.eps)
+
+
+class GatedFeedForward(nn.Module):
+    """Channel-mixing block of a residual stream on pixel-major maps:
+
+        n = N_pre(x),  h = W_down (act(W_gate n) * (W_up n)),  y = x + scale * gate * dropout(N_post(h))
+
+    `n` and `next_norm` chain blocks: the junction of one block also computes the next one's normalised input.  Norms of a
+    chain share their kind and eps."""
+
+    def __init__(self, dim, hidden, act='silu', norm='rms', p=0.0, bias=False, post=True, scale=None, eps=1e-5):
+        super().__init__()
+        self.act, self.norm, self.eps, self.p, self.rng = act, norm, eps, p, None
+        self.pre = RowNorm(dim, norm, eps)
+        self.gate_proj = nn.Conv2d(dim, hidden, 1, bias=bias)
+        self.up_proj = nn.Conv2d(dim, hidden, 1, bias=bias)
+        self.down_proj = nn.Conv2d(hidden, dim, 1, bias=bias)
+        self.post = RowNorm(dim, norm, eps) if post else None
+        self.scale = nn.Parameter(torch.full((dim,), float(scale))) if scale is not None else None
+
+    def forward(self, x, n=None, gate=None, next_norm=None):
+        """-> (y, next_norm(y) or None); n: this block's normalised input where the block before computed it; gate [N, dim]"""
+        if next_norm is not None and (next_norm.norm, next_norm.eps) != (self.norm, self.eps):
+            raise ValueError(f'a chain of {self.norm} norms with eps {self.eps}, then {next_norm.norm} with {next_norm.eps}')
+        n = self.pre(x) if n is None else n
+        z = Fh.gated_linear(n, self.gate_proj.weight, self.up_proj.weight, self.gate_proj.bias, self.up_proj.bias, self.act)
+        h = run_conv(z, self.down_proj)
+        wb = lambda m: None if m is None else (m.weight, m.bias)
+        return Fh.norm_residual(x, h, gate=gate, scale=self.scale, post=wb(self.post), pre=wb(next_norm), norm=self.norm, eps=self.eps, p=self.p,
+                                training=self.training, rng=self.rng)
+
+
+class GatedFeedForwardTrunk(nn.Module):
+    """`depth` GatedFeedForward blocks, one junction kernel between two of them; kwargs as GatedFeedForward's"""
+
+    def __init__(self, depth, dim, hidden, **kwargs):
+        super().__init__()
+        self.blocks = nn.ModuleList(GatedFeedForward(dim, hidden, **kwargs) for _ in range(depth))
+
+    def forward(self, x, gate=None):
+        n = None
+        for i, b in enumerate(self.blocks):
+            x, n = b(x, n, gate, self.blocks[i + 1].pre if i + 1 < len(self.blocks) else None)
+        return x

@@ -1,0 +1,186 @@
+"""The transformer-block operators without a GPU: the 64-bit oracle against published vectors, autograd and differences; every call that
+the Python surface and the C ABI refuse."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import transformer_ops as O
+
+
+def test_philox_known_answers():
+    """the test vectors published with the generator (Random123, philox4x32-10)"""
+    f = 0xffffffff
+    for counter, key, want in (((0, 0, 0, 0), (0, 0), (0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8)),
+                               ((f, f, f, f), (f, f), (0x408f276d, 0x41c83b0e, 0xa20bc7c6, 0x6d5451fd)),
+                               ((0x243f6a88, 0x85a308d3, 0x13198a2e, 0x03707344), (0xa4093822, 0x299f31d0),
+                                (0xd16cfe09, 0x94fdcceb, 0x5001e420, 0x24126ea1))):
+        got = O.philox4x32(np.array([counter], dtype=np.uint64), key)[0]
+        assert tuple(int(v) for v in got) == want
+
+
+def test_keep_mask_windows_and_rate():
+    full = O.keep_mask(100_000, O.threshold_of(0.3), 7, 1 << 40)
+    assert torch.equal(full[1237:5000], O.keep_mask(5000 - 1237, O.threshold_of(0.3), 7, 1 << 40, first=1237))
+    rate = 1 - float(full.double().mean())
+    assert abs(rate - 0.3) < 5 * (0.3 * 0.7 / 100_000) ** 0.5
+    far = O.keep_mask(64, 1 << 15, 3, 9, first=(1 << 35) + 3)               # element indexes beyond 32 bits move the second counter word
+    assert not torch.equal(far, O.keep_mask(64, 1 << 15, 3, 9, first=3))
+
+
+def _rnd(*shape, seed):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed), dtype=torch.float64)
+
+
+@pytest.mark.parametrize('layer', [False, True])
+@pytest.mark.parametrize('post,pre,gated,p', [(True, True, True, 0.25), (False, True, False, 0.0), (True, False, True, 0.0), (False, False, False, 0.5)])
+def test_oracle_norm_residual_gradients(layer, post, pre, gated, p):
+    N, H, W, C = 2, 2, 3, 5
+    x, h, dy, dn = (_rnd(N, H, W, C, seed=i) for i in range(4))
+    gate, scale = (_rnd(N, C, seed=5), _rnd(C, seed=6)) if gated else (None, None)
+    post = (_rnd(C, seed=7), _rnd(C, seed=8)) if post else None
+    pre = (_rnd(C, seed=9), _rnd(C, seed=10)) if pre else None
+    leaves = dict(x=x, h=h, gate=gate, scale=scale, post_w=post and post[0], post_b=post and post[1], pre_w=pre and pre[0], pre_b=pre and pre[1])
+    leaves = {k: v.clone().requires_grad_(True) for k, v in leaves.items() if v is not None}
+
+    def loss(v):
+        from torch.nn import functional as F
+
+        def norm(t, w, b):
+            return F.layer_norm(t, (C,), w, b, 1e-5) if layer else F.rms_norm(t, (C,), w, 1e-5) + b
+        u = norm(v['h'], v['post_w'], v['post_b']) if post else v['h']
+        if p:
+            u = u * O.dropout(torch.ones(N, H, W, C), p, 11, 12)
+        for k in ('scale', 'gate'):
+            if k in v:
+                u = u * (v[k].view(N, 1, 1, C) if k == 'gate' else v[k])
+        y = v['x'] + u
+        return (y * dy).sum() + ((norm(y, v['pre_w'], v['pre_b']) * dn).sum() if pre else 0)
+
+    got = O.norm_residual(x, h, dy, dn if pre else None, gate, scale, post, pre, layer, 1e-5, p, 11, 12)
+    want = torch.autograd.grad(loss(leaves), list(leaves.values()))
+    for (k, v), w in zip(leaves.items(), want):
+        assert torch.allclose(got[k][0], w, rtol=1e-10, atol=1e-10), k
+        e = torch.zeros_like(v.detach()).view(-1)                          # a central difference along one coordinate: error O(eps^2)
+        e[0] = 1e-5
+        e = e.view(v.shape)
+        dif = (loss({**leaves, k: v + e}) - loss({**leaves, k: v - e})) / 2e-5
+        assert abs(float(dif) - float(w.reshape(-1)[0])) < 1e-6 * (1 + abs(float(dif))), k
+
+
+@pytest.mark.parametrize('name', ['silu', 'gelu', 'sigmoid', 'relu'])
+def test_oracle_gated_linear_gradients(name):
+    M, K, F = 5, 4, 6
+    v = [_rnd(*s, seed=i).requires_grad_(True) for i, s in enumerate([(M, K), (F, K), (F, K), (F,), (F,)])]
+    dz = _rnd(M, F, seed=9)
+    fn = dict(silu=torch.nn.functional.silu, gelu=torch.nn.functional.gelu, sigmoid=torch.sigmoid, relu=torch.relu)[name]
+
+    def value(x, wg, wu, bg, bu):
+        return fn(x @ wg.t() + bg) * (x @ wu.t() + bu)
+    got = O.gated_linear(*(t.detach() for t in v), dz, name, 0.0)
+    assert torch.allclose(got['z'][0], value(*v), rtol=1e-10, atol=1e-12)
+    for k, w in zip(('x', 'wg', 'wu', 'bg', 'bu'), torch.autograd.grad(value(*v), v, dz)):
+        assert torch.allclose(got[k][0], w, rtol=1e-10, atol=1e-10), k
+    assert torch.autograd.gradcheck(value, v)
+
+
+# ---- refusals -------------------------------------------------------------------------------------------------------------
+def test_dropout_refusals():
+    from rdfc_gan_amd import functional as Fh
+    x = torch.zeros(1, 2, 3, 8)
+    for bad in (torch.zeros(2, 8), torch.zeros(1, 2, 3, 0), 3):
+        with pytest.raises(ValueError):
+            Fh.dropout(bad, 0.5, rng=(1, 2))
+    with pytest.raises(TypeError):
+        Fh.dropout(x.double(), 0.5, rng=(1, 2))
+    for p in (-0.1, 1.1, float('nan')):
+        with pytest.raises(ValueError, match='probability'):
+            Fh.dropout(x, p, rng=(1, 2))
+    for rng in ((-1, 0), (0, 1 << 64)):
+        with pytest.raises(ValueError, match='64-bit'):
+            Fh.dropout(x, 0.5, rng=rng)
+    for rng in (None, (1, 2)):
+        with pytest.raises(ValueError, match='device'):
+            Fh.dropout(x, 0.5, rng=rng)
+    assert Fh.dropout(x, 0.5, training=False) is x and Fh.dropout(x, 0.0) is x and Fh.dropout(x, 1e-6) is x
+
+
+def test_norm_residual_refusals():
+    from rdfc_gan_amd import functional as Fh
+    x = torch.zeros(2, 2, 3, 8)
+    w = torch.ones(8)
+    for kw in (dict(h=torch.zeros(2, 2, 3, 7)), dict(h=x.half()), dict(gate=torch.ones(8)), dict(gate=torch.ones(2, 3, 8)), dict(scale=torch.ones(7)),
+               dict(post=(torch.ones(7), None)), dict(pre=(w, torch.ones(9))), dict(norm='batch', pre=(w, None)), dict(eps=-1.0), dict(p=2.0),
+               dict(scale=torch.ones(8, dtype=torch.int32)), dict()):
+        with pytest.raises(ValueError):
+            Fh.norm_residual(x, kw.pop('h', x), **kw)
+    wide = torch.zeros(1, 1, 1, 8193)
+    with pytest.raises(ValueError, match='8192'):
+        Fh.norm_residual(wide, wide)
+    with pytest.raises(ValueError, match='8192'):
+        Fh.row_norm(wide)
+    with pytest.raises(ValueError):
+        Fh.row_norm(x, torch.ones(9))
+    with pytest.raises(ValueError, match='device'):
+        Fh.row_norm(x, w)
+
+
+def test_gated_linear_refusals():
+    from rdfc_gan_amd import functional as Fh
+    x, w = torch.zeros(1, 2, 3, 8), torch.zeros(5, 8)
+    b = torch.zeros(5)
+    for args, kw in (((w, torch.zeros(6, 8)), {}), ((torch.zeros(5, 7),) * 2, {}), ((torch.zeros(0, 8),) * 2, {}), ((torch.zeros(5, 8, 3, 3),) * 2, {}),
+                     ((w, w, b), {}), ((w, w, b, torch.zeros(4)), {}), ((w, w), dict(act='tanh')), ((w.half(), w.half()), {}), ((w, w.half()), {}),
+                     ((torch.zeros(8),) * 2, {}), ((w, w, b, b), {})):
+        with pytest.raises(ValueError):
+            Fh.gated_linear(x, *args, **kw)
+    with pytest.raises(ValueError, match='device'):
+        Fh.gated_linear(x, w, w)
+
+
+def test_c_abi_refusals():
+    from rdfc_gan_amd import hip
+    lib = hip.lib()
+    err = lambda: lib.rdfc_last_error()
+    assert lib.rdfc_dropout(None, None, 4, 8, 8, 8, 0, 65537, 0, 0, None, None) and b'threshold' in err()
+    assert lib.rdfc_dropout(None, None, 4, 8, 7, 8, 0, 5, 0, 0, None, None) and b'bad sizes' in err()
+    assert lib.rdfc_dropout(None, None, 4, 8, 8, 8, 3, 5, 0, 0, None, None) and b'dtype' in err()
+    assert lib.rdfc_dropout(None, None, 4, 8, 8, 8, 0, 5, 0, 0, None, None) and b'null' in err()
+    assert lib.rdfc_dropout(None, None, 0, 8, 8, 8, 0, 5, 0, 0, None, None) == 0
+    assert lib.rdfc_dropout_draw(None, None, None)
+    nr = lambda **k: hip.NormResidualDesc(**{**dict(rows=4, samples=2, C=8, ldx=8, ldh=8, dtype=0, pre=1, eps=1e-5), **k})
+    fwd = lambda d: lib.rdfc_norm_residual(ctypes.byref(d), *[None] * 13)
+    assert fwd(nr()) and b'null' in err()
+    assert fwd(nr(C=8193, ldx=9000, ldh=9000)) and b'8192' in err()
+    assert fwd(nr(ldx=7)) and b'ld smaller' in err()
+    assert fwd(nr(threshold=-1)) and b'threshold' in err()
+    assert fwd(nr(samples=70000)) and b'bad sizes' in err()
+    assert fwd(nr(rows=0)) == 0
+    assert lib.rdfc_norm_residual_scratch_floats(ctypes.byref(nr(C=0)), 0) == 0
+    bwd = lambda d, lddy=8, lddn=8: lib.rdfc_norm_residual_backward(ctypes.byref(d), *[None] * 9, None, lddy, None, lddn, *[None] * 10)
+    assert bwd(nr()) and b'null' in err()
+    assert bwd(nr(rows=0)) == 0
+    gl = lambda **k: hip.GatedDesc(**{**dict(M=4, K=8, F=8, ldx=8, ldwg=8, ldwu=8, dtype=1, act=16), **k})
+    fwd = lambda d: lib.rdfc_gated_linear(ctypes.byref(d), *[None] * 7)
+    assert fwd(gl()) and b'null' in err()
+    assert fwd(gl(act=2)) and b'activation' in err()
+    assert fwd(gl(ldwu=4)) and b'ld smaller' in err()
+    assert fwd(gl(K=0)) and b'bad sizes' in err()
+    assert fwd(gl(F=(1 << 20) + 1)) and b'bad sizes' in err()
+    assert fwd(gl(M=0)) == 0
+    assert lib.rdfc_gated_linear_scratch_bytes(ctypes.byref(gl(dtype=9))) == 0
+    bwd = lambda d, lddz=8, dw=0: lib.rdfc_gated_linear_backward(ctypes.byref(d), *[None] * 6, lddz, None, None, None, None, dw, None, None, None)
+    assert bwd(gl()) and b'null' in err()
+    assert bwd(gl(), lddz=7) and b'lddz' in err()
+    assert bwd(gl(), dw=2) and b'weight gradients' in err()
+
+
+def test_residual_block_with_dropout_has_upstream_indices():
+    """use_dropout puts nn.Dropout(0.5) behind the first activation: the second convolution is conv_block.6"""
+    from rdfc_gan_amd.generator import ResnetGenerator
+    g = ResnetGenerator(1, 3, ngf=8, norm_layer='IN2d', use_dropout=True, n_blocks=1)
+    keys = [k for k in g.state_dict() if 'conv_block' in k]
+    assert {k.split('conv_block.')[1] for k in keys} == {'1.weight', '1.bias', '6.weight', '6.bias'}
+    plain = ResnetGenerator(1, 3, ngf=8, norm_layer='IN2d', n_blocks=1)
+    assert {k.split('conv_block.')[1] for k in plain.state_dict() if 'conv_block' in k} == {'1.weight', '1.bias', '5.weight', '5.bias'}

@@ -582,10 +582,13 @@ typedef struct rdfc_gated_desc {
     int64_t M;
     int32_t K, F, ldx, ldwg, ldwu, dtype, act;
 } rdfc_gated_desc;
-int rdfc_gated_linear(const rdfc_gated_desc *d, const void *x, const void *wg, const void *wu, const float *bg, const float *bu, void *z, void *stream);
-size_t rdfc_gated_linear_scratch_bytes(const rdfc_gated_desc *d);
+/* bytes of scratch (256-byte aligned) that a forward or backward call with these operands needs; the pointers' alignment counts, not what
+ * they point to: rows that are not whole 16-byte vectors are copied first.  0: scratch may be NULL. */
+size_t rdfc_gated_linear_scratch_bytes(const rdfc_gated_desc *d, const void *x, const void *wg, const void *wu, int backward);
+int rdfc_gated_linear(const rdfc_gated_desc *d, const void *x, const void *wg, const void *wu, const float *bg, const float *bu, void *scratch,
+                      void *z, void *stream);
 /* dz [M][F] (lddz) -> dx dense [M][K], dwg, dwu dense [F][K] (dw_dtype: RDFC_F32 or the map's type), dbg, dbu f32 [F]; each may be NULL.
- * scratch: 256-byte aligned.  g and u are computed again; dg and du are rounded to the map's type for the two products, the bias gradients
+ * g and u are computed again; dg and du are rounded to the map's type for the two products, the bias gradients
  * are summed before that.  Sums have a fixed order. */
 int rdfc_gated_linear_backward(const rdfc_gated_desc *d, const void *x, const void *wg, const void *wu, const float *bg, const float *bu, const void *dz,
                                int lddz, void *scratch, void *dx, void *dwg, void *dwu, int dw_dtype, float *dbg, float *dbu, void *stream);

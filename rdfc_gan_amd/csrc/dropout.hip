@@ -5,27 +5,86 @@
 
 namespace {
 
-constexpr int NT = 256, GPT = 4;      // threads, groups of eight elements per thread
+constexpr int NT = 256;
 
-// Groups of eight consecutive elements of the dense order.  VECTOR: every group lies inside a row and is 16-byte aligned in x and y.
-template <typename T, bool VECTOR>
+template <typename T> struct Eight {               // eight consecutive elements: one 16-byte vector, two in f32
+    static constexpr int NV = 8 / Elem<T>::VEC;
+    Vec16<T> v[NV];
+    __device__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i].load(p + i * Elem<T>::VEC);
+    }
+    __device__ void store(T *p) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i].store(p + i * Elem<T>::VEC);
+    }
+    __device__ float get(int i) const { return v[i / Elem<T>::VEC].get(i % Elem<T>::VEC); }
+    __device__ void set(int i, float f) { v[i / Elem<T>::VEC].set(i % Elem<T>::VEC, f); }
+};
+
+// Groups of eight consecutive elements of the dense order, GPT per thread, all their loads in flight before the first mask is drawn.
+//   FLAT     x and y are dense: a group is at 8 q in both
+//   ROWS     C is a multiple of 8 and every row 16-byte aligned: a group lies inside a row
+//   ANY      everything else: element by element
+// WIDE: element indexes of 64 bits (the division by C costs about three times a 32-bit one)
+enum { FLAT, ROWS, ANY };
+template <typename T, int HOW, int GPT, bool WIDE>
 __global__ __launch_bounds__(NT) void dropout_kernel(DropArgs d, const T *__restrict__ x, T *__restrict__ y, unsigned long long n, int C, int ldx, int ldy) {
+    using I = typename std::conditional<WIDE, unsigned long long, unsigned>::type;
     const unsigned long long seed = d.key ? d.key[0] : d.seed, offset = d.key ? d.key[1] : d.offset;
-    const unsigned long long ngroups = (n + 7) >> 3, g0 = (unsigned long long)blockIdx.x * (NT * GPT) + threadIdx.x;
-    for (int k = 0; k < GPT; ++k) {
-        const unsigned long long q = g0 + k * NT;
-        if (q >= ngroups) return;
-        unsigned long long row = (q << 3) / (unsigned)C;
-        int c = (int)((q << 3) - row * (unsigned)C);
-        const unsigned keep = keep8(q << 3, d.threshold, seed, offset);
-        for (int i = 0; i < 8 && (q << 3) + i < n; ++i) {
-            const float v = Elem<T>::ld(x + row * (unsigned)ldx + c);
-            Elem<T>::st(y + row * (unsigned)ldy + c, keep >> i & 1 ? v * d.inv : 0.f);
-            if (++c == C) {
+    const I ngroups = (I)((n + 7) >> 3), g0 = (I)blockIdx.x * (NT * GPT) + threadIdx.x;
+    if constexpr (HOW != ANY) {
+        Eight<T> v[GPT];
+        unsigned long long dst[GPT];
+#pragma unroll
+        for (int k = 0; k < GPT; ++k) {
+            const I q = g0 + k * NT;
+            if (q < ngroups) {
+                unsigned long long src = (unsigned long long)q << 3;
+                dst[k] = src;
+                if constexpr (HOW == ROWS) {
+                    const I row = q / (unsigned)(C >> 3);
+                    const unsigned c = (unsigned)(q - row * (unsigned)(C >> 3)) << 3;
+                    src = (unsigned long long)row * (unsigned)ldx + c;
+                    dst[k] = (unsigned long long)row * (unsigned)ldy + c;
+                }
+                v[k].load(x + src);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < GPT; ++k) {
+            const I q = g0 + k * NT;
+            if (q >= ngroups) break;
+            const u32x4 w = philox(q, seed, offset);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[k].set(i, word16(w, i) >= d.threshold ? v[k].get(i) * d.inv : 0.f);
+            v[k].store(y + dst[k]);
+        }
+    } else {
+        static_assert(HOW != ANY || GPT == 1, "one group a thread where elements move one by one");
+        if (g0 >= ngroups) return;
+        const unsigned long long e0 = (unsigned long long)g0 << 3;
+        unsigned long long row;
+        unsigned c;
+        if (WIDE) row = e0 / (unsigned)C;
+        else row = (unsigned)e0 / (unsigned)C;
+        c = (unsigned)(e0 - row * (unsigned)C);
+        const int m = n - e0 < 8 ? (int)(n - e0) : 8;
+        float v[8];
+        unsigned long long dst[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            dst[i] = row * (unsigned)ldy + c;
+            v[i] = i < m ? Elem<T>::ld(x + row * (unsigned)ldx + c) : 0.f;
+            if (++c == (unsigned)C) {
                 c = 0;
                 ++row;
             }
         }
+        const u32x4 w = philox(g0, seed, offset);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < m) Elem<T>::st(y + dst[i], word16(w, i) >= d.threshold ? v[i] * d.inv : 0.f);
     }
 }
 
@@ -45,9 +104,27 @@ extern "C" int rdfc_dropout(const void *x, void *y, int64_t P, int C, int ldx, i
     RDFC_REQUIRE(drop_args(d, threshold, seed, offset, key), "rdfc_dropout: threshold %d is not in [0, 65536]", threshold);
     if (P == 0) return 0;
     RDFC_REQUIRE(x && y, "rdfc_dropout: null map");
-    const unsigned long long n = (unsigned long long)P * C, blocks = ((n + 7) / 8 + NT * GPT - 1) / (NT * GPT);
+    const unsigned long long n = (unsigned long long)P * C, groups = (n + 7) / 8;
+    const int vec = rdfc_vec(dtype);
+    const bool al = ((reinterpret_cast<size_t>(x) | reinterpret_cast<size_t>(y)) & 15) == 0;
+    // (a dense map with a last group that is not whole goes element by element)
+    const int how = al && ldx == C && ldy == C && n % 8 == 0 ? FLAT : al && C % 8 == 0 && ldx % vec == 0 && ldy % vec == 0 ? ROWS : ANY;
+    const int gpt = how == ANY ? 1 : groups >= 256 * 2048 ? 4 : 1;
+    const unsigned long long blocks = (groups + NT * gpt - 1) / (NT * gpt);
+    const bool wide = n + 8ull * NT * gpt >= 1ull << 32;
     RDFC_REQUIRE(blocks < (1ull << 31), "rdfc_dropout: %llu elements are too many", n);
-    RDFC_DISPATCH(dtype, (dropout_kernel<T, false><<<dim3((unsigned)blocks), NT, 0, (hipStream_t)stream>>>(d, (const T *)x, (T *)y, n, C, ldx, ldy)));
+    auto go = [&](auto h, auto g, auto w) {
+        constexpr int H = decltype(h)::value, G = decltype(g)::value;
+        constexpr bool W = decltype(w)::value;
+        RDFC_DISPATCH(dtype, (dropout_kernel<T, H, G, W><<<dim3((unsigned)blocks), NT, 0, (hipStream_t)stream>>>(d, (const T *)x, (T *)y, n, C, ldx, ldy)));
+    };
+    auto pick = [&](auto w) {
+        if (how == FLAT) gpt == 4 ? go(std::integral_constant<int, FLAT>{}, std::integral_constant<int, 4>{}, w) : go(std::integral_constant<int, FLAT>{}, std::integral_constant<int, 1>{}, w);
+        else if (how == ROWS) gpt == 4 ? go(std::integral_constant<int, ROWS>{}, std::integral_constant<int, 4>{}, w) : go(std::integral_constant<int, ROWS>{}, std::integral_constant<int, 1>{}, w);
+        else go(std::integral_constant<int, ANY>{}, std::integral_constant<int, 1>{}, w);
+    };
+    if (wide) pick(std::true_type{});
+    else pick(std::false_type{});
     RDFC_LAUNCH_CHECK("rdfc_dropout");
     return 0;
 }

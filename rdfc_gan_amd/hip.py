@@ -53,7 +53,7 @@ def lib():
         _lib.rdfc_last_kernel.restype = C.c_char_p
         _lib.rdfc_build_hash.restype = C.c_char_p
         _lib.rdfc_norm_residual_scratch_floats.argtypes, _lib.rdfc_norm_residual_scratch_floats.restype = [C.c_void_p, C.c_int], C.c_size_t
-        _lib.rdfc_gated_linear_scratch_bytes.argtypes, _lib.rdfc_gated_linear_scratch_bytes.restype = [C.c_void_p], C.c_size_t
+        _lib.rdfc_gated_linear_scratch_bytes.argtypes, _lib.rdfc_gated_linear_scratch_bytes.restype = [C.c_void_p] * 4 + [C.c_int], C.c_size_t
         _declare_argtypes(_lib)
     return _lib
 
@@ -1124,6 +1124,11 @@ def norm_residual_backward(d, x, h, gate, scale, post, pre, key, stats, dy, dn, 
     return (dx, dh, *cols)
 
 
+def _gated_scratch(d, x, wg, wu, backward):
+    n = lib().rdfc_gated_linear_scratch_bytes(C.byref(d), _p(x), _p(wg), _p(wu), backward)
+    return torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+
+
 def gated_linear(x, wg, wu, bg, bu, act):
     """-> (descriptor, z); x pixel-major, weights [F, K] rows of the map's type"""
     N, H, W, K = x.shape
@@ -1131,7 +1136,8 @@ def gated_linear(x, wg, wu, bg, bu, act):
     d = GatedDesc(N * H * W, K, F, ld(x), wg.stride(0) if F > 1 else K, wu.stride(0) if F > 1 else K, dt(x), GATE_ACT[act])
     z = torch.empty(N, H, W, F, dtype=x.dtype, device=x.device)
     if z.numel():
-        _call('rdfc_gated_linear', x, C.byref(d), _p(x), _p(wg), _p(wu), _p(bg), _p(bu), _p(z))
+        scratch = _gated_scratch(d, x, wg, wu, 0)
+        _call('rdfc_gated_linear', x, C.byref(d), _p(x), _p(wg), _p(wu), _p(bg), _p(bu), _p(scratch), _p(z))
     return d, z
 
 
@@ -1142,7 +1148,7 @@ def gated_linear_backward(d, x, wg, wu, bg, bu, dz, want_dx, dw_dtype, want_bias
     dx = torch.empty(N, H, W, K, dtype=x.dtype, device=x.device) if want_dx else None
     dwg, dwu = (torch.empty(F, K, dtype=dw_dtype, device=x.device) for _ in range(2)) if dw_dtype is not None else (None, None)
     dbg, dbu = (torch.empty(F, dtype=torch.float32, device=x.device) for _ in range(2)) if want_bias else (None, None)
-    scratch = torch.empty(lib().rdfc_gated_linear_scratch_bytes(C.byref(d)), dtype=torch.uint8, device=x.device)
+    scratch = _gated_scratch(d, x, wg, wu, 1)
     _call('rdfc_gated_linear_backward', x, C.byref(d), _p(x), _p(wg), _p(wu), _p(bg), _p(bu), _p(dz), ld(dz), _p(scratch), _p(dx), _p(dwg), _p(dwu),
           F32 if dw_dtype == torch.float32 else dt(x), _p(dbg), _p(dbu))
     return dx, dwg, dwu, dbg, dbu

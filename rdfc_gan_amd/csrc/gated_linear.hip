@@ -232,11 +232,22 @@ __global__ __launch_bounds__(NT, 2) void gated_dma_kernel(GLArgs p, int tiles_p,
         }
     };
 
+    // (GATED: rows alternate 16 features of the gate with 16 of the other projection, and the accumulators start at the biases)
     f32x4 acc[MT][QT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < MT; ++i) {
+        f32x4 first = {0, 0, 0, 0};
+        if constexpr (GATED) {
+            const float *bias = i & 1 ? p.bu : p.bg;
+            const int f = p0 + wp * (WTP / 2) + 16 * (i >> 1) + 4 * (lane >> 4);
+            if (bias != nullptr) {
 #pragma unroll
-        for (int j = 0; j < QT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+                for (int r = 0; r < 4; ++r) first[r] = f + r < p.F ? bias[f + r] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < QT; ++j) acc[i][j] = first;
+    }
 
     // ---- fragments: 16 rows (or columns) from `first`, the step's whole contraction range ---------------------------------------------
     const int l16 = lane & 15, g4 = lane >> 4;
@@ -341,16 +352,6 @@ __global__ __launch_bounds__(NT, 2) void gated_dma_kernel(GLArgs p, int tiles_p,
     };
     if constexpr (GATED) {
         const int fw = p0 + wp * OW;                             // the wave's first feature
-        float bg[MT / 2][4], bu[MT / 2][4];
-#pragma unroll
-        for (int i = 0; i < MT / 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int f = fw + 16 * i + q4 + r;
-                const bool on = p.bg != nullptr && f < p.F;
-                bg[i][r] = on ? p.bg[f] : 0.f;
-                bu[i][r] = on ? p.bu[f] : 0.f;
-            }
         with_gate(p.act, [&](auto act) {
             constexpr int ACT = decltype(act)::value;
             if constexpr (MODE == FWD) {
@@ -363,8 +364,8 @@ __global__ __launch_bounds__(NT, 2) void gated_dma_kernel(GLArgs p, int tiles_p,
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             float a, da;
-                            gate_act<ACT, ES == 4>(acc[2 * i][j][r] + bg[i][r], a, da);
-                            v[r] = a * (acc[2 * i + 1][j][r] + bu[i][r]);
+                            gate_act<ACT, ES == 4>(acc[2 * i][j][r], a, da);
+                            v[r] = a * acc[2 * i + 1][j][r];
                         }
                         put(16 * i + q4, v);
                     }
@@ -381,6 +382,7 @@ __global__ __launch_bounds__(NT, 2) void gated_dma_kernel(GLArgs p, int tiles_p,
                 for (int j = 0; j < QT; ++j) {
                     const int64_t m = q0 + wq * WTQ + 16 * j + l16;
                     float w[MT / 2][4];
+                    __builtin_amdgcn_sched_barrier(0);           // (or every j's dz is fetched at once, and the accumulators spill)
 #pragma unroll
                     for (int i = 0; i < MT / 2; ++i) {
                         const int f = fw + 16 * i + q4;
@@ -405,10 +407,10 @@ __global__ __launch_bounds__(NT, 2) void gated_dma_kernel(GLArgs p, int tiles_p,
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             float a, da;
-                            gate_act<ACT, ES == 4>(acc[2 * i][j][r] + bg[i][r], a, da);
+                            gate_act<ACT, ES == 4>(acc[2 * i][j][r], a, da);
                             // (a pixel or feature that is not there: zero, whatever its accumulators hold)
                             const bool on = m < p.M && f + r < p.F;
-                            v[r] = on ? dz[r] * (acc[2 * i + 1][j][r] + bu[i][r]) * da : 0.f;
+                            v[r] = on ? dz[r] * acc[2 * i + 1][j][r] * da : 0.f;
                             w[i][r] = on ? dz[r] * a : 0.f;
                             sg[i][r] += v[r];
                             su[i][r] += w[i][r];
@@ -482,6 +484,23 @@ template <typename TO> __global__ __launch_bounds__(NT) void gated_join_kernel(c
     double s = 0.;
     for (int k = 0; k < parts; ++k) s += (double)partial[k * step + src];
     Elem<TO>::st(o + i, (float)s);
+}
+
+// out[kind][f] = sum over the row blocks of partial[block][kind * Fp + f]: 32 columns x 16 row lanes per workgroup
+__global__ __launch_bounds__(512) void gated_bias_kernel(const float *__restrict__ partial, int blocks, int F, int Fp, float *__restrict__ o0, float *__restrict__ o1) {
+    __shared__ double red[16][32];
+    const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;      // (2 Fp is a multiple of 64)
+    double s = 0.;
+#pragma unroll 8
+    for (int k = rl; k < blocks; k += 16) s += (double)partial[(size_t)k * 2 * Fp + c];
+    red[rl][cl] = s;
+    __syncthreads();
+    if (rl != 0) return;
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += red[k][cl];
+    const int kind = c >= Fp, f = kind ? c - Fp : c;
+    float *o = kind ? o1 : o0;
+    if (o != nullptr && f < F) o[f] = (float)s;
 }
 
 // what the kernel needs of an operand: rows of whole 16-byte vectors, and offsets of a tile that fit 31 bits
@@ -681,7 +700,7 @@ extern "C" int rdfc_gated_linear_backward(const rdfc_gated_desc *d, const void *
     }
     // (M = 0: no parts, zeros)
     if (dbg || dbu) {
-        gated_join_kernel<float><<<dim3(cdiv(d->F, NT), 2), NT, 0, st>>>(bias, row_blocks, d->F, q.Fp, 1, dbg, dbu);
+        gated_bias_kernel<<<2 * q.Fp / 32, 512, 0, st>>>(bias, row_blocks, d->F, q.Fp, dbg, dbu);
         RDFC_LAUNCH_CHECK("rdfc_gated_linear_backward (bias join)");
     }
     if (dwg || dwu) {

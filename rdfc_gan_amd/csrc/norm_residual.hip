@@ -39,6 +39,8 @@ struct NRArgs {
 };
 
 // ---- sums over the LPR lanes that own a row ------------------------------------------------------------------------------
+// All of it in vector registers (DPP inside 16 lanes, permlane swaps above): a shuffle through LDS has several times the latency, and a
+// row's pass waits for up to four sums in turn.
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
     return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
@@ -47,8 +49,16 @@ template <int LPR> __device__ __forceinline__ float lanes_sum(float v) {
     v = dpp_add<0x4E>(v);                                        // quad_perm 2,3,0,1
     v = dpp_add<0x141>(v);                                       // row_half_mirror: eight lanes
     if constexpr (LPR >= 16) v = dpp_add<0x140>(v);              // row_mirror
-    if constexpr (LPR >= 32) v += __shfl_xor(v, 16, 64);
-    if constexpr (LPR >= 64) v += __shfl_xor(v, 32, 64);
+    if constexpr (LPR >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+        const unsigned r0 = r[0], r1 = r[1];                     // (a bit cast of r[1] itself reads r[0])
+        v = __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
+    }
+    if constexpr (LPR >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+        const unsigned r0 = r[0], r1 = r[1];                     // (a bit cast of r[1] itself reads r[0])
+        v = __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
+    }
     return v;
 }
 // two sums at once.  LPR = 256: over the workgroup, through LDS (`buf`: two slots of 8 floats used in turn; every thread calls)
@@ -69,29 +79,31 @@ template <int LPR> __device__ __forceinline__ void row_sum2(float &a, float &b, 
 }
 
 // ---- eight channels ------------------------------------------------------------------------------------------------------
-// ALIGNED: C is a multiple of 8 and every row 16-byte aligned
-template <typename T, bool ALIGNED> __device__ __forceinline__ void load8(float (&v)[8], const T *row, int c, int C) {
-    if constexpr (ALIGNED) {
-        if (c >= C) {
+// as they lie in memory, so that a row can be fetched while the one before it is worked on.  ALIGNED: C is a multiple of 8 and every
+// row 16-byte aligned
+template <typename T, bool ALIGNED> struct Raw8 {
+    static constexpr int NV = sizeof(T) / 2;
+    Vec16<T> v[NV];
+    __device__ __forceinline__ void load(const T *row, int c, int C) {
+        if constexpr (ALIGNED) {
+            if (c < C) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.f;
-        } else if constexpr (sizeof(T) == 4) {
-            Vec16<T> a, b;
-            a.load(row + c);
-            b.load(row + c + 4);
+                for (int i = 0; i < NV; ++i) v[i].load(row + c + i * Elem<T>::VEC);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = a.get(i), v[4 + i] = b.get(i);
+                for (int i = 0; i < NV; ++i) v[i].zero();
+            }
         } else {
-            Vec16<T> a;
-            a.load(row + c);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = a.get(i);
+            for (int i = 0; i < 8; ++i) v[i / Elem<T>::VEC].set(i % Elem<T>::VEC, c + i < C ? Elem<T>::ld(row + c + i) : 0.f);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < C ? Elem<T>::ld(row + c + i) : 0.f;
     }
-}
+    __device__ __forceinline__ float get(int i) const { return v[i / Elem<T>::VEC].get(i % Elem<T>::VEC); }
+    __device__ __forceinline__ void get8(float (&f)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = get(i);
+    }
+};
 template <typename T, bool ALIGNED> __device__ __forceinline__ void store8(const float (&v)[8], T *row, int c, int C) {
     if constexpr (ALIGNED) {
         if (c >= C) return;
@@ -170,15 +182,27 @@ __global__ __launch_bounds__(NT) void norm_residual_kernel(NRArgs p) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) a[v][i] *= rstd;
     };
-    for (int64_t r = r0 + threadIdx.x / LPR; r < r1; r += RPB) {
+    Raw8<T, ALIGNED> nx[VPL], nh[VPL];                            // the next row
+    auto fetch = [&](int64_t r) {
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) {
+            nx[v].load((const T *)p.x + (base + r) * p.ldx, (v * LPR + li) * 8, C);
+            if (p.h != nullptr) nh[v].load((const T *)p.h + (base + r) * p.ldh, (v * LPR + li) * 8, C);
+        }
+    };
+    int64_t r = r0 + threadIdx.x / LPR;
+    if (r < r1) fetch(r);
+    for (; r < r1; r += RPB) {
         const int64_t row = base + r;
         float a[VPL][8], b[VPL][8];
 #pragma unroll
-        for (int v = 0; v < VPL; ++v) load8<T, ALIGNED>(a[v], (const T *)p.x + row * p.ldx, (v * LPR + li) * 8, C);
+        for (int v = 0; v < VPL; ++v) {
+            nx[v].get8(a[v]);
+            if (p.h != nullptr) nh[v].get8(b[v]);
+        }
+        if (r + RPB < r1) fetch(r + RPB);
         f32x4 st = {0.f, 0.f, 0.f, 0.f};
         if (p.h != nullptr) {
-#pragma unroll
-            for (int v = 0; v < VPL; ++v) load8<T, ALIGNED>(b[v], (const T *)p.h + row * p.ldh, (v * LPR + li) * 8, C);
             if (p.post) {
                 float m, s;
                 normalise(b, m, s);
@@ -264,19 +288,41 @@ __global__ __launch_bounds__(NT) void norm_residual_bwd_kernel(NRArgs p) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) g[v][i] = rstd * (g[v][i] - fmaf(hat[v][i], s, z));
     };
-    for (int64_t r = r0 + grp; r < r1; r += RPB) {
+    Raw8<T, ALIGNED> nx[VPL], nh[VPL], ny[VPL], nn[VPL];          // the next row
+    f32x4 nst = {0.f, 0.f, 0.f, 0.f};
+    auto fetch = [&](int64_t r) {
+        nst = p.stats[base + r];
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) {
+            const int c = (v * LPR + li) * 8;
+            nx[v].load((const T *)p.x + (base + r) * p.ldx, c, C);
+            if (p.h != nullptr) nh[v].load((const T *)p.h + (base + r) * p.ldh, c, C);
+            if (p.dy != nullptr) ny[v].load((const T *)p.dy + (base + r) * p.lddy, c, C);
+            if (p.dn != nullptr) nn[v].load((const T *)p.dn + (base + r) * p.lddn, c, C);
+        }
+    };
+    int64_t r = r0 + grp;
+    if (r < r1) fetch(r);
+    for (; r < r1; r += RPB) {
         const int64_t row = base + r;
         float a[VPL][8], hat[VPL][8], t[VPL][8];
+        Raw8<T, ALIGNED> dy[VPL];
         unsigned keep[VPL];
-        const f32x4 st = p.stats[row];
+        const f32x4 st = nst;
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) {
+            nx[v].get8(a[v]);
+            if (p.h != nullptr) nh[v].get8(hat[v]);
+            if (p.dn != nullptr) nn[v].get8(t[v]);
+            if (p.dy != nullptr) dy[v] = ny[v];
+        }
+        if (r + RPB < r1) fetch(r + RPB);
         // hat = normalised h (or h), a = y
 #pragma unroll
         for (int v = 0; v < VPL; ++v) {
             const int c = (v * LPR + li) * 8;
-            load8<T, ALIGNED>(a[v], (const T *)p.x + row * p.ldx, c, C);
             keep[v] = 0xff;
             if (p.h != nullptr) {
-                load8<T, ALIGNED>(hat[v], (const T *)p.h + row * p.ldh, c, C);
                 if (p.drop.threshold != 0) keep[v] = keep8((unsigned long long)row * C + c, p.drop.threshold, seed, offset);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -294,7 +340,6 @@ __global__ __launch_bounds__(NT) void norm_residual_bwd_kernel(NRArgs p) {
 #pragma unroll
             for (int v = 0; v < VPL; ++v) {
                 const int c = (v * LPR + li) * 8;
-                load8<T, ALIGNED>(t[v], (const T *)p.dn + row * p.lddn, c, C);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     a[v][i] = c + i < C ? (a[v][i] - st[2]) * st[3] : 0.f;
@@ -314,10 +359,8 @@ __global__ __launch_bounds__(NT) void norm_residual_bwd_kernel(NRArgs p) {
         for (int v = 0; v < VPL; ++v) {
             const int c = (v * LPR + li) * 8;
             if (p.dy != nullptr) {
-                float d[8];
-                load8<T, ALIGNED>(d, (const T *)p.dy + row * p.lddy, c, C);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t[v][i] += d[i];
+                for (int i = 0; i < 8; ++i) t[v][i] += dy[v].get(i);
             }
             store8<T, ALIGNED>(t[v], (T *)p.dx + row * C, c, C);
         }
@@ -366,47 +409,54 @@ __global__ __launch_bounds__(NT) void norm_residual_bwd_kernel(NRArgs p) {
     }
 }
 
-// ---- column sums: 16 channels x 16 chunk lanes per workgroup --------------------------------------------------------------------
+// ---- column sums ---------------------------------------------------------------------------------------------------------
+// Two small kernels.  First, 64 columns x 8 row lanes per workgroup over PARTS slices of a sample's partial rows (one workgroup per
+// column tile alone reads 256 B of every row: at 20 GB/s a CU a thousand rows took 30 us); then one thread per channel.
 struct NRGrads {
     float *gate, *scale, *post_w, *post_b, *pre_w, *pre_b;       // each may be null
 };
-__global__ __launch_bounds__(NT) void norm_residual_cols_kernel(NRArgs p, NRGrads o, int samples, int nchunk) {
-    __shared__ double red[16][4][17];
-    const int cl = threadIdx.x & 15, kl = threadIdx.x >> 4, C = p.C, c = blockIdx.x * 16 + cl;
+constexpr int SUM_COLS = 64, SUM_ROWS = 8, SLICE = 64;           // partial rows per workgroup
+__global__ __launch_bounds__(SUM_COLS * SUM_ROWS) void norm_residual_sum_kernel(const float *__restrict__ partial, double *__restrict__ sums, int cols, int nchunk) {
+    __shared__ double red[SUM_ROWS][SUM_COLS];
+    const int cl = threadIdx.x % SUM_COLS, rl = threadIdx.x / SUM_COLS, c = blockIdx.x * SUM_COLS + cl;
+    const int k0 = blockIdx.z * SLICE, k1 = min(k0 + SLICE, nchunk);
+    double s = 0.;
+    if (c < cols) {
+        const float *src = partial + (size_t)blockIdx.y * nchunk * cols + c;
+#pragma unroll 8
+        for (int k = k0 + rl; k < k1; k += SUM_ROWS) s += (double)src[(size_t)k * cols];
+    }
+    red[rl][cl] = s;
+    __syncthreads();
+    if (rl != 0 || c >= cols) return;
+#pragma unroll
+    for (int k = 1; k < SUM_ROWS; ++k) s += red[k][cl];
+    sums[((size_t)blockIdx.y * gridDim.z + blockIdx.z) * cols + c] = s;
+}
+__global__ __launch_bounds__(64) void norm_residual_grads_kernel(NRArgs p, NRGrads o, const double *__restrict__ sums, int samples, int slices) {
+    const int C = p.C, c = blockIdx.x * 64 + threadIdx.x;
+    if (c >= C) return;
+    const double sc = p.scale ? p.scale[c] : 1., w = p.post ? (p.post_w ? p.post_w[c] : 1.) : 1., b = p.post && p.post_b ? p.post_b[c] : 0.;
     double dscale = 0., dpw = 0., dpb = 0., dqw = 0., dqb = 0.;
     for (int g = 0; g < samples; ++g) {
         double s[4] = {0., 0., 0., 0.};
-        if (c < C)
-            for (int k = kl; k < nchunk; k += 16)
+#pragma unroll 4
+        for (int k = 0; k < slices; ++k)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[j] += (double)p.partial[(((size_t)g * nchunk + k) * 4 + j) * C + c];
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) red[kl][j][cl] = s[j];
-        __syncthreads();
-        if (kl == 0 && c < C) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                s[j] = 0.;
-                for (int k = 0; k < 16; ++k) s[j] += red[k][j][cl];
-            }
-            const double sc = p.scale ? p.scale[c] : 1., gt = p.gate ? p.gate[(size_t)g * C + c] : 1.;
-            const double S = p.post ? (p.post_w ? p.post_w[c] : 1.) * s[0] + (p.post_b ? p.post_b[c] : 0.) * s[1] : s[0];
-            if (o.gate) o.gate[(size_t)g * C + c] = (float)(sc * S);
-            dscale += gt * S;
-            dpw += sc * gt * s[0];
-            dpb += sc * gt * s[1];
-            dqw += s[2];
-            dqb += s[3];
-        }
+            for (int j = 0; j < 4; ++j) s[j] += sums[(((size_t)g * slices + k) * 4 + j) * C + c];
+        const double gt = p.gate ? p.gate[(size_t)g * C + c] : 1., S = w * s[0] + b * s[1];
+        if (o.gate) o.gate[(size_t)g * C + c] = (float)(sc * S);
+        dscale += gt * S;
+        dpw += sc * gt * s[0];
+        dpb += sc * gt * s[1];
+        dqw += s[2];
+        dqb += s[3];
     }
-    if (kl == 0 && c < C) {
-        if (o.scale) o.scale[c] = (float)dscale;
-        if (o.post_w) o.post_w[c] = (float)dpw;
-        if (o.post_b) o.post_b[c] = (float)dpb;
-        if (o.pre_w) o.pre_w[c] = (float)dqw;
-        if (o.pre_b) o.pre_b[c] = (float)dqb;
-    }
+    if (o.scale) o.scale[c] = (float)dscale;
+    if (o.post_w) o.post_w[c] = (float)dpw;
+    if (o.post_b) o.post_b[c] = (float)dpb;
+    if (o.pre_w) o.pre_w[c] = (float)dqw;
+    if (o.pre_b) o.pre_b[c] = (float)dqb;
 }
 
 constexpr int MAXC = 8192;
@@ -427,14 +477,28 @@ int lanes_of(int C) {
     with_layout(C, [&](auto lpr, auto) { l = decltype(lpr)::value; });
     return l;
 }
-// rows per workgroup: about 1024 workgroups, each row group at least four rows (the backward kernel leaves 4 C sums per workgroup)
-int64_t chunk_of(int64_t rows, int samples, int C) {
+// rows per workgroup: about `groups` workgroups in all (the backward kernel leaves 4 C sums per workgroup)
+int64_t chunk_of(int64_t rows, int samples, int C, int groups) {
     const int64_t rpb = NT / lanes_of(C), total = rows * samples;
-    int64_t per = (total + 1023) / 1024;
-    per = per < 4 * rpb ? 4 * rpb : per;
+    int64_t per = (total + groups - 1) / groups;
     per = (per + rpb - 1) / rpb * rpb;
     while ((rows + per - 1) / per >= (1 << 20)) per *= 2;
     return per;
+}
+constexpr int FWD_GROUPS = 2048, BWD_GROUPS = 1024;
+struct NRChunks {
+    int64_t chunk;
+    int nchunk, slices;
+    size_t partial, sums;            // floats of the partial rows (even), doubles of their sums
+};
+NRChunks bwd_chunks(int64_t rows, int samples, int C) {
+    NRChunks k;
+    k.chunk = chunk_of(rows, samples, C, BWD_GROUPS);
+    k.nchunk = (int)((rows + k.chunk - 1) / k.chunk);
+    k.slices = (k.nchunk + SLICE - 1) / SLICE;
+    k.partial = (size_t)samples * k.nchunk * 4 * C;
+    k.sums = (size_t)samples * k.slices * 4 * C;
+    return k;
 }
 bool row_aligned(const void *p, int ld, int dtype) { return (reinterpret_cast<size_t>(p) & 15) == 0 && ld % rdfc_vec(dtype) == 0; }
 
@@ -486,7 +550,7 @@ extern "C" int rdfc_norm_residual(const rdfc_norm_residual_desc *d, const void *
     // (without a gate the samples are one run of rows)
     const int samples = gate ? d->samples : 1;
     p.rows = gate ? d->rows : d->rows * d->samples;
-    p.chunk = chunk_of(p.rows, samples, d->C);
+    p.chunk = chunk_of(p.rows, samples, d->C, FWD_GROUPS);
     const dim3 grid((unsigned)((p.rows + p.chunk - 1) / p.chunk), samples);
     const bool al = row_aligned(x, d->ldx, d->dtype) && row_aligned(h, d->ldh, d->dtype) && row_aligned(y, d->C, d->dtype) && row_aligned(n, d->C, d->dtype) && d->C % 8 == 0;
     with_layout(d->C, [&](auto lpr, auto vpl) {
@@ -501,8 +565,8 @@ extern "C" int rdfc_norm_residual(const rdfc_norm_residual_desc *d, const void *
 extern "C" size_t rdfc_norm_residual_scratch_floats(const rdfc_norm_residual_desc *d, int gated) {
     if (nr_check(d, "rdfc_norm_residual_scratch_floats") || d->samples == 0 || d->rows == 0) return 0;
     const int samples = gated ? d->samples : 1;
-    const int64_t rows = gated ? d->rows : d->rows * d->samples, chunk = chunk_of(rows, samples, d->C);
-    return (size_t)samples * (size_t)((rows + chunk - 1) / chunk) * 4 * d->C;
+    const NRChunks k = bwd_chunks(gated ? d->rows : d->rows * d->samples, samples, d->C);
+    return k.partial + 2 * k.sums;
 }
 
 extern "C" int rdfc_norm_residual_backward(const rdfc_norm_residual_desc *d, const void *x, const void *h, const float *gate, const float *scale,
@@ -527,12 +591,12 @@ extern "C" int rdfc_norm_residual_backward(const rdfc_norm_residual_desc *d, con
     p.stats = reinterpret_cast<f32x4 *>(const_cast<float *>(stats));
     p.partial = cols ? scratch : nullptr;
     const int samples = gate ? d->samples : 1;
-    int nchunk = 0;
+    NRChunks k = {};
     if (!empty) {
         p.rows = gate ? d->rows : d->rows * d->samples;
-        p.chunk = chunk_of(p.rows, samples, d->C);
-        nchunk = (int)((p.rows + p.chunk - 1) / p.chunk);
-        const dim3 grid((unsigned)nchunk, samples);
+        k = bwd_chunks(p.rows, samples, d->C);
+        p.chunk = k.chunk;
+        const dim3 grid((unsigned)k.nchunk, samples);
         const bool al = row_aligned(x, d->ldx, d->dtype) && row_aligned(h, d->ldh, d->dtype) && row_aligned(dy, lddy, d->dtype) &&
                         row_aligned(dn, lddn, d->dtype) && row_aligned(dx, d->C, d->dtype) && row_aligned(dh, d->C, d->dtype) && d->C % 8 == 0;
         with_layout(d->C, [&](auto lpr, auto vpl) {
@@ -544,7 +608,10 @@ extern "C" int rdfc_norm_residual_backward(const rdfc_norm_residual_desc *d, con
     }
     if (cols) {
         const NRGrads o = {d_gate, d_scale, d_post_w, d_post_b, d_pre_w, d_pre_b};
-        norm_residual_cols_kernel<<<cdiv(d->C, 16), NT, 0, (hipStream_t)stream>>>(p, o, samples, nchunk);
+        double *sums = reinterpret_cast<double *>(scratch + k.partial);         // (8-byte aligned: partial is a multiple of 4)
+        if (!empty)
+            norm_residual_sum_kernel<<<dim3(cdiv(4 * d->C, SUM_COLS), samples, k.slices), SUM_COLS * SUM_ROWS, 0, (hipStream_t)stream>>>(scratch, sums, 4 * d->C, k.nchunk);
+        norm_residual_grads_kernel<<<cdiv(d->C, 64), 64, 0, (hipStream_t)stream>>>(p, o, sums, samples, k.slices);
         RDFC_LAUNCH_CHECK("rdfc_norm_residual_backward (columns)");
     }
     return 0;

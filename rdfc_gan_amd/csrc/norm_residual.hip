@@ -18,9 +18,13 @@
 // bits every run.
 #include "philox.h"
 
+#include <initializer_list>
+
 namespace {
 
-constexpr int NT = 256;
+// threads of a workgroup: four waves, or the two that share a row of up to 1024 channels (one vector a lane keeps the backward kernel at three
+// waves per SIMD; two vectors a lane of one wave need 300 registers)
+constexpr int threads_of(int lpr) { return lpr == 128 ? 128 : 256; }
 
 struct NRArgs {
     const void *x, *h;
@@ -44,24 +48,29 @@ struct NRArgs {
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
     return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
+// v of a lane + v of the lane W away (lane ^ W)
+template <int W> __device__ __forceinline__ float halves_sum(float v) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    unsigned r0, r1;                                             // (taken apart first: a bit cast of the vector's element 1 reads element 0)
+    if constexpr (W == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        r0 = r[0], r1 = r[1];
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        r0 = r[0], r1 = r[1];
+    }
+    return __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
+}
 template <int LPR> __device__ __forceinline__ float lanes_sum(float v) {
     v = dpp_add<0xB1>(v);                                        // quad_perm 1,0,3,2
     v = dpp_add<0x4E>(v);                                        // quad_perm 2,3,0,1
     v = dpp_add<0x141>(v);                                       // row_half_mirror: eight lanes
     if constexpr (LPR >= 16) v = dpp_add<0x140>(v);              // row_mirror
-    if constexpr (LPR >= 32) {
-        const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
-        const unsigned r0 = r[0], r1 = r[1];                     // (a bit cast of r[1] itself reads r[0])
-        v = __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
-    }
-    if constexpr (LPR >= 64) {
-        const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
-        const unsigned r0 = r[0], r1 = r[1];                     // (a bit cast of r[1] itself reads r[0])
-        v = __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
-    }
+    if constexpr (LPR >= 32) v = halves_sum<16>(v);
+    if constexpr (LPR >= 64) v = halves_sum<32>(v);
     return v;
 }
-// two sums at once.  LPR = 256: over the workgroup, through LDS (`buf`: two slots of 8 floats used in turn; every thread calls)
+// two sums at once.  LPR > 64: over the workgroup, through LDS (`buf`: two slots of 8 floats used in turn; every thread calls)
 template <int LPR> __device__ __forceinline__ void row_sum2(float &a, float &b, float (*buf)[8], int &turn) {
     a = lanes_sum<LPR>(a);
     b = lanes_sum<LPR>(b);
@@ -73,8 +82,8 @@ template <int LPR> __device__ __forceinline__ void row_sum2(float &a, float &b, 
             s[4 + (threadIdx.x >> 6)] = b;
         }
         __syncthreads();                                         // (the other slot is not written again before the next barrier)
-        a = (s[0] + s[1]) + (s[2] + s[3]);
-        b = (s[4] + s[5]) + (s[6] + s[7]);
+        a = LPR == 128 ? s[0] + s[1] : (s[0] + s[1]) + (s[2] + s[3]);
+        b = LPR == 128 ? s[4] + s[5] : (s[4] + s[5]) + (s[6] + s[7]);
     }
 }
 
@@ -125,34 +134,49 @@ template <typename T, bool ALIGNED> __device__ __forceinline__ void store8(const
             if (c + i < C) Elem<T>::st(row + c + i, v[i]);
     }
 }
-// a parameter vector (f32, any alignment); a null pointer stands for `none`.  0 beyond C: what the lanes behind the last channel hold must
-// not enter a sum
-__device__ __forceinline__ void load_par(float (&v)[8], const float *p, int c, int C, float none) {
+// a parameter vector (f32); a null pointer stands for `none`.  0 beyond C: what the lanes behind the last channel hold must not enter a sum
+template <bool ALIGNED> __device__ __forceinline__ void load_par(float (&v)[8], const float *p, int c, int C, float none) {
+    if (ALIGNED && p != nullptr && c < C) {
+        const f32x4 a = *reinterpret_cast<const f32x4 *>(p + c), b = *reinterpret_cast<const f32x4 *>(p + c + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = c + i >= C ? 0.f : p != nullptr ? p[c + i] : none;
 }
+// y = x + D (fw hhat + fb): fw = scale gate w_post, fb = scale gate b_post
+template <int LPR, int VPL, bool ALIGNED> __device__ __forceinline__ void load_factors(const NRArgs &p, int li, float (&fw)[VPL][8], float (&fb)[VPL][8]) {
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+        const int c = (v * LPR + li) * 8;
+        float s[8], g[8];
+        load_par<ALIGNED>(s, p.scale, c, p.C, 1.f);
+        load_par<ALIGNED>(g, p.gate ? p.gate + (size_t)blockIdx.y * p.C : nullptr, c, p.C, 1.f);
+        load_par<ALIGNED>(fw[v], p.post_w, c, p.C, 1.f);
+        load_par<ALIGNED>(fb[v], p.post_b, c, p.C, 0.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            fw[v][i] *= s[i] * g[i];
+            fb[v][i] *= s[i] * g[i];
+        }
+    }
+}
 
 template <typename T, int LPR, int VPL, bool ALIGNED>
-__global__ __launch_bounds__(NT) void norm_residual_kernel(NRArgs p) {
-    constexpr int RPB = NT / LPR;
+__global__ __launch_bounds__(threads_of(LPR), VPL == 1 ? (sizeof(T) == 2 ? 5 : 4) : 1) void norm_residual_kernel(NRArgs p) {
+    constexpr int NT = threads_of(LPR), RPB = NT / LPR;
     __shared__ float buf[2][8];
     int turn = 0;
     const int li = threadIdx.x % LPR, C = p.C;
     const float rC = 1.f / (float)C;
     const unsigned long long seed = p.drop.key ? p.drop.key[0] : p.drop.seed, offset = p.drop.key ? p.drop.key[1] : p.drop.offset;
-    float f[VPL][8], pw[VPL][8], pb[VPL][8], qw[VPL][8], qb[VPL][8];
+    float fw[VPL][8], fb[VPL][8], qw[VPL][8], qb[VPL][8];
+    load_factors<LPR, VPL, ALIGNED>(p, li, fw, fb);
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
-        const int c = (v * LPR + li) * 8;
-        float g[8];
-        load_par(f[v], p.scale, c, C, 1.f);
-        load_par(g, p.gate ? p.gate + (size_t)blockIdx.y * C : nullptr, c, C, 1.f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[v][i] *= g[i];
-        load_par(pw[v], p.post_w, c, C, 1.f);
-        load_par(pb[v], p.post_b, c, C, 0.f);
-        load_par(qw[v], p.pre_w, c, C, 1.f);
-        load_par(qb[v], p.pre_b, c, C, 0.f);
+        load_par<ALIGNED>(qw[v], p.pre_w, (v * LPR + li) * 8, C, 1.f);
+        load_par<ALIGNED>(qb[v], p.pre_b, (v * LPR + li) * 8, C, 0.f);
     }
     const int64_t r0 = (int64_t)blockIdx.x * p.chunk, r1 = min(r0 + p.chunk, p.rows), base = (int64_t)blockIdx.y * p.rows;
     // mean and reciprocal deviation of the row in a[][]; a[][] becomes the normalised row
@@ -190,11 +214,24 @@ __global__ __launch_bounds__(NT) void norm_residual_kernel(NRArgs p) {
             if (p.h != nullptr) nh[v].load((const T *)p.h + (base + r) * p.ldh, (v * LPR + li) * 8, C);
         }
     };
+    // the row's mask, drawn before its data is touched: the multiplications run while the loads are under way
+    auto draw = [&](int64_t row, unsigned (&keep)[VPL]) {
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) {
+            keep[v] = 0xff;
+            if (p.drop.threshold != 0) {
+                keep[v] = keep8<ALIGNED>((unsigned long long)row * C + (v * LPR + li) * 8, p.drop.threshold, seed, offset);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
     int64_t r = r0 + threadIdx.x / LPR;
     if (r < r1) fetch(r);
     for (; r < r1; r += RPB) {
         const int64_t row = base + r;
         float a[VPL][8], b[VPL][8];
+        unsigned keep[VPL];
+        draw(row, keep);
 #pragma unroll
         for (int v = 0; v < VPL; ++v) {
             nx[v].get8(a[v]);
@@ -212,17 +249,10 @@ __global__ __launch_bounds__(NT) void norm_residual_kernel(NRArgs p) {
 #pragma unroll
             for (int v = 0; v < VPL; ++v) {
                 const int c = (v * LPR + li) * 8;
-                if (p.post) {
+                // (a dropped element stays out whatever its value: no 0 * inf)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) b[v][i] = fmaf(b[v][i], pw[v][i], pb[v][i]);
-                }
-                if (p.drop.threshold != 0) {
-                    const unsigned keep = keep8((unsigned long long)row * C + c, p.drop.threshold, seed, offset);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) b[v][i] = keep >> i & 1 ? b[v][i] * p.drop.inv : 0.f;
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) a[v][i] = fmaf(f[v][i], b[v][i], a[v][i]);
+                for (int i = 0; i < 8; ++i)
+                    if (keep[v] >> i & 1) a[v][i] = fmaf(fmaf(b[v][i], fw[v][i], fb[v][i]), p.drop.inv, a[v][i]);
                 store8<T, ALIGNED>(a[v], (T *)p.y + row * p.ldy, c, C);
             }
         }
@@ -243,27 +273,20 @@ __global__ __launch_bounds__(NT) void norm_residual_kernel(NRArgs p) {
 }
 
 template <typename T, int LPR, int VPL, bool ALIGNED>
-__global__ __launch_bounds__(NT) void norm_residual_bwd_kernel(NRArgs p) {
-    constexpr int RPB = NT / LPR;
+__global__ __launch_bounds__(threads_of(LPR), VPL == 1 ? (sizeof(T) == 2 ? 3 : 2) : 1) void norm_residual_bwd_kernel(NRArgs p) {
+    constexpr int NT = threads_of(LPR), RPB = NT / LPR;
     __shared__ float buf[2][8];
-    __shared__ float red[RPB > 1 ? (RPB / 2) * LPR * VPL * 8 : 1];
+    __shared__ float red[LPR <= 64 ? 4 : 1][LPR <= 64 ? LPR * VPL * 8 : 1];
     int turn = 0;
     const int li = threadIdx.x % LPR, grp = threadIdx.x / LPR, C = p.C;
     const float rC = 1.f / (float)C;
     const unsigned long long seed = p.drop.key ? p.drop.key[0] : p.drop.seed, offset = p.drop.key ? p.drop.key[1] : p.drop.offset;
-    float f[VPL][8], pw[VPL][8], pb[VPL][8], qw[VPL][8];
+    float fw[VPL][8], fb[VPL][8], qw[VPL][8];
     float sum[4][VPL][8];                                        // A, B, P, Q
+    load_factors<LPR, VPL, ALIGNED>(p, li, fw, fb);
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
-        const int c = (v * LPR + li) * 8;
-        float g[8];
-        load_par(f[v], p.scale, c, C, 1.f);
-        load_par(g, p.gate ? p.gate + (size_t)blockIdx.y * C : nullptr, c, C, 1.f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[v][i] *= g[i];
-        load_par(pw[v], p.post_w, c, C, 1.f);
-        load_par(pb[v], p.post_b, c, C, 0.f);
-        load_par(qw[v], p.pre_w, c, C, 1.f);
+        load_par<ALIGNED>(qw[v], p.pre_w, (v * LPR + li) * 8, C, 1.f);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -301,6 +324,17 @@ __global__ __launch_bounds__(NT) void norm_residual_bwd_kernel(NRArgs p) {
             if (p.dn != nullptr) nn[v].load((const T *)p.dn + (base + r) * p.lddn, c, C);
         }
     };
+    // the row's mask, drawn before its data is touched: the multiplications run while the loads are under way
+    auto draw = [&](int64_t row, unsigned (&keep)[VPL]) {
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) {
+            keep[v] = 0xff;
+            if (p.drop.threshold != 0) {
+                keep[v] = keep8<ALIGNED>((unsigned long long)row * C + (v * LPR + li) * 8, p.drop.threshold, seed, offset);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
     int64_t r = r0 + grp;
     if (r < r1) fetch(r);
     for (; r < r1; r += RPB) {
@@ -308,6 +342,7 @@ __global__ __launch_bounds__(NT) void norm_residual_bwd_kernel(NRArgs p) {
         float a[VPL][8], hat[VPL][8], t[VPL][8];
         Raw8<T, ALIGNED> dy[VPL];
         unsigned keep[VPL];
+        draw(row, keep);
         const f32x4 st = nst;
 #pragma unroll
         for (int v = 0; v < VPL; ++v) {
@@ -321,17 +356,11 @@ __global__ __launch_bounds__(NT) void norm_residual_bwd_kernel(NRArgs p) {
 #pragma unroll
         for (int v = 0; v < VPL; ++v) {
             const int c = (v * LPR + li) * 8;
-            keep[v] = 0xff;
             if (p.h != nullptr) {
-                if (p.drop.threshold != 0) keep[v] = keep8((unsigned long long)row * C + c, p.drop.threshold, seed, offset);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    float u = hat[v][i];
-                    if (p.post) {
-                        hat[v][i] = c + i < C ? (hat[v][i] - st[0]) * st[1] : 0.f;
-                        u = fmaf(hat[v][i], pw[v][i], pb[v][i]);
-                    }
-                    a[v][i] = fmaf(f[v][i], keep[v] >> i & 1 ? u * p.drop.inv : 0.f, a[v][i]);
+                    if (p.post) hat[v][i] = c + i < C ? (hat[v][i] - st[0]) * st[1] : 0.f;
+                    if (keep[v] >> i & 1) a[v][i] = fmaf(fmaf(hat[v][i], fw[v][i], fb[v][i]), p.drop.inv, a[v][i]);
                 }
             }
         }
@@ -372,39 +401,42 @@ __global__ __launch_bounds__(NT) void norm_residual_bwd_kernel(NRArgs p) {
                 const float d = keep[v] >> i & 1 ? t[v][i] * p.drop.inv : 0.f;
                 sum[0][v][i] = fmaf(d, hat[v][i], sum[0][v][i]);
                 sum[1][v][i] += d;
-                t[v][i] = d * f[v][i] * pw[v][i];
+                t[v][i] = d * fw[v][i];
             }
         if (p.post) through(t, hat, st[1]);
 #pragma unroll
         for (int v = 0; v < VPL; ++v) store8<T, ALIGNED>(t[v], (T *)p.dh + row * C, (v * LPR + li) * 8, C);
     }
-    // the row groups' sums, halved until one is left, then one partial row per sum: partial[sample][chunk][4][C]
+    // the row groups' sums: those of a wave in its registers, the four waves' in LDS, one partial row per sum: partial[sample][chunk][4][C]
     if (p.partial == nullptr) return;
     float *out = p.partial + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 * C;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        for (int half = RPB / 2; half > 0; half >>= 1) {
-            __syncthreads();
-            if (grp >= half && grp < 2 * half) {
-#pragma unroll
-                for (int v = 0; v < VPL; ++v)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) red[((grp - half) * LPR + li) * (VPL * 8) + v * 8 + i] = sum[k][v][i];
-            }
-            __syncthreads();
-            if (grp < half) {
-#pragma unroll
-                for (int v = 0; v < VPL; ++v)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) sum[k][v][i] += red[(grp * LPR + li) * (VPL * 8) + v * 8 + i];
-            }
-        }
-        if (grp == 0) {
+        if constexpr (LPR > 64) {
 #pragma unroll
             for (int v = 0; v < VPL; ++v)
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if ((v * LPR + li) * 8 + i < C) out[(size_t)k * C + (v * LPR + li) * 8 + i] = sum[k][v][i];
+        } else {
+            if (k) __syncthreads();
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float &s = sum[k][v][i];
+                    if constexpr (LPR <= 8) s = dpp_add<0x128>(s);           // row_ror:8
+                    if constexpr (LPR <= 16) s = halves_sum<16>(s);
+                    if constexpr (LPR <= 32) s = halves_sum<32>(s);
+                }
+                if ((threadIdx.x & 63) < LPR) {
+                    f32x4 *dst = reinterpret_cast<f32x4 *>(&red[threadIdx.x >> 6][(v * LPR + li) * 8]);
+                    dst[0] = f32x4{sum[k][v][0], sum[k][v][1], sum[k][v][2], sum[k][v][3]};
+                    dst[1] = f32x4{sum[k][v][4], sum[k][v][5], sum[k][v][6], sum[k][v][7]};
+                }
+            }
+            __syncthreads();
+            for (int c = threadIdx.x; c < C; c += NT) out[(size_t)k * C + c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
         }
     }
 }
@@ -415,7 +447,7 @@ __global__ __launch_bounds__(NT) void norm_residual_bwd_kernel(NRArgs p) {
 struct NRGrads {
     float *gate, *scale, *post_w, *post_b, *pre_w, *pre_b;       // each may be null
 };
-constexpr int SUM_COLS = 64, SUM_ROWS = 8, SLICE = 64;           // partial rows per workgroup
+constexpr int SUM_COLS = 64, SUM_ROWS = 8, SLICE = 128;          // partial rows per workgroup
 __global__ __launch_bounds__(SUM_COLS * SUM_ROWS) void norm_residual_sum_kernel(const float *__restrict__ partial, double *__restrict__ sums, int cols, int nchunk) {
     __shared__ double red[SUM_ROWS][SUM_COLS];
     const int cl = threadIdx.x % SUM_COLS, rl = threadIdx.x / SUM_COLS, c = blockIdx.x * SUM_COLS + cl;
@@ -433,30 +465,37 @@ __global__ __launch_bounds__(SUM_COLS * SUM_ROWS) void norm_residual_sum_kernel(
     for (int k = 1; k < SUM_ROWS; ++k) s += red[k][cl];
     sums[((size_t)blockIdx.y * gridDim.z + blockIdx.z) * cols + c] = s;
 }
-__global__ __launch_bounds__(64) void norm_residual_grads_kernel(NRArgs p, NRGrads o, const double *__restrict__ sums, int samples, int slices) {
-    const int C = p.C, c = blockIdx.x * 64 + threadIdx.x;
-    if (c >= C) return;
-    const double sc = p.scale ? p.scale[c] : 1., w = p.post ? (p.post_w ? p.post_w[c] : 1.) : 1., b = p.post && p.post_b ? p.post_b[c] : 0.;
-    double dscale = 0., dpw = 0., dpb = 0., dqw = 0., dqb = 0.;
-    for (int g = 0; g < samples; ++g) {
-        double s[4] = {0., 0., 0., 0.};
+// 64 channels x 8 sample lanes
+__global__ __launch_bounds__(512) void norm_residual_grads_kernel(NRArgs p, NRGrads o, const double *__restrict__ sums, int samples, int slices) {
+    __shared__ double red[8][5][64];
+    const int C = p.C, cl = threadIdx.x & 63, gl = threadIdx.x >> 6, c = blockIdx.x * 64 + cl;
+    double acc[5] = {0., 0., 0., 0., 0.};                        // scale, post_w, post_b, pre_w, pre_b
+    if (c < C) {
+        const double sc = p.scale ? p.scale[c] : 1., w = p.post && p.post_w ? p.post_w[c] : 1., b = p.post && p.post_b ? p.post_b[c] : 0.;
+        for (int g = gl; g < samples; g += 8) {
+            double s[4] = {0., 0., 0., 0.};
 #pragma unroll 4
-        for (int k = 0; k < slices; ++k)
+            for (int k = 0; k < slices; ++k)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] += sums[(((size_t)g * slices + k) * 4 + j) * C + c];
-        const double gt = p.gate ? p.gate[(size_t)g * C + c] : 1., S = w * s[0] + b * s[1];
-        if (o.gate) o.gate[(size_t)g * C + c] = (float)(sc * S);
-        dscale += gt * S;
-        dpw += sc * gt * s[0];
-        dpb += sc * gt * s[1];
-        dqw += s[2];
-        dqb += s[3];
+                for (int j = 0; j < 4; ++j) s[j] += sums[(((size_t)g * slices + k) * 4 + j) * C + c];
+            const double gt = p.gate ? p.gate[(size_t)g * C + c] : 1., S = w * s[0] + b * s[1];
+            if (o.gate) o.gate[(size_t)g * C + c] = (float)(sc * S);
+            acc[0] += gt * S;
+            acc[1] += sc * gt * s[0];
+            acc[2] += sc * gt * s[1];
+            acc[3] += s[2];
+            acc[4] += s[3];
+        }
     }
-    if (o.scale) o.scale[c] = (float)dscale;
-    if (o.post_w) o.post_w[c] = (float)dpw;
-    if (o.post_b) o.post_b[c] = (float)dpb;
-    if (o.pre_w) o.pre_w[c] = (float)dqw;
-    if (o.pre_b) o.pre_b[c] = (float)dqb;
+#pragma unroll
+    for (int k = 0; k < 5; ++k) red[gl][k][cl] = acc[k];
+    __syncthreads();
+    if (gl >= 5 || c >= C) return;
+    double s = 0.;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += red[k][gl][cl];
+    float *out = gl == 0 ? o.scale : gl == 1 ? o.post_w : gl == 2 ? o.post_b : gl == 3 ? o.pre_w : o.pre_b;
+    if (out) out[c] = (float)s;
 }
 
 constexpr int MAXC = 8192;
@@ -467,7 +506,7 @@ template <typename F> void with_layout(int C, F &&f) {
     else if (nv <= 16) f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
     else if (nv <= 32) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
     else if (nv <= 64) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
-    else if (nv <= 128) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+    else if (nv <= 128) f(std::integral_constant<int, 128>{}, std::integral_constant<int, 1>{});
     else if (nv <= 256) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
     else if (nv <= 512) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
     else f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
@@ -479,13 +518,15 @@ int lanes_of(int C) {
 }
 // rows per workgroup: about `groups` workgroups in all (the backward kernel leaves 4 C sums per workgroup)
 int64_t chunk_of(int64_t rows, int samples, int C, int groups) {
-    const int64_t rpb = NT / lanes_of(C), total = rows * samples;
+    const int lpr = lanes_of(C), nt = threads_of(lpr);
+    const int64_t rpb = nt / lpr, total = rows * samples;
+    groups *= 256 / nt;
     int64_t per = (total + groups - 1) / groups;
     per = (per + rpb - 1) / rpb * rpb;
     while ((rows + per - 1) / per >= (1 << 20)) per *= 2;
     return per;
 }
-constexpr int FWD_GROUPS = 2048, BWD_GROUPS = 1024;
+constexpr int FWD_GROUPS = 1280, BWD_GROUPS = 768;
 struct NRChunks {
     int64_t chunk;
     int nchunk, slices;
@@ -499,6 +540,11 @@ NRChunks bwd_chunks(int64_t rows, int samples, int C) {
     k.partial = (size_t)samples * k.nchunk * 4 * C;
     k.sums = (size_t)samples * k.slices * 4 * C;
     return k;
+}
+bool par_aligned(std::initializer_list<const float *> ps) {
+    size_t a = 0;
+    for (const float *p : ps) a |= reinterpret_cast<size_t>(p);
+    return a % 16 == 0;
 }
 bool row_aligned(const void *p, int ld, int dtype) { return (reinterpret_cast<size_t>(p) & 15) == 0 && ld % rdfc_vec(dtype) == 0; }
 
@@ -552,11 +598,12 @@ extern "C" int rdfc_norm_residual(const rdfc_norm_residual_desc *d, const void *
     p.rows = gate ? d->rows : d->rows * d->samples;
     p.chunk = chunk_of(p.rows, samples, d->C, FWD_GROUPS);
     const dim3 grid((unsigned)((p.rows + p.chunk - 1) / p.chunk), samples);
-    const bool al = row_aligned(x, d->ldx, d->dtype) && row_aligned(h, d->ldh, d->dtype) && row_aligned(y, d->C, d->dtype) && row_aligned(n, d->C, d->dtype) && d->C % 8 == 0;
+    const bool al = row_aligned(x, d->ldx, d->dtype) && row_aligned(h, d->ldh, d->dtype) && row_aligned(y, d->C, d->dtype) && row_aligned(n, d->C, d->dtype) && d->C % 8 == 0 &&
+                    par_aligned({gate, scale, post_w, post_b, pre_w, pre_b});
     with_layout(d->C, [&](auto lpr, auto vpl) {
         constexpr int L = decltype(lpr)::value, V = decltype(vpl)::value;
-        RDFC_DISPATCH(d->dtype, if (al) norm_residual_kernel<T, L, V, true><<<grid, NT, 0, (hipStream_t)stream>>>(p);
-                      else norm_residual_kernel<T, L, V, false><<<grid, NT, 0, (hipStream_t)stream>>>(p));
+        RDFC_DISPATCH(d->dtype, if (al) norm_residual_kernel<T, L, V, true><<<grid, threads_of(L), 0, (hipStream_t)stream>>>(p);
+                      else norm_residual_kernel<T, L, V, false><<<grid, threads_of(L), 0, (hipStream_t)stream>>>(p));
     });
     RDFC_LAUNCH_CHECK("rdfc_norm_residual");
     return 0;
@@ -598,11 +645,12 @@ extern "C" int rdfc_norm_residual_backward(const rdfc_norm_residual_desc *d, con
         p.chunk = k.chunk;
         const dim3 grid((unsigned)k.nchunk, samples);
         const bool al = row_aligned(x, d->ldx, d->dtype) && row_aligned(h, d->ldh, d->dtype) && row_aligned(dy, lddy, d->dtype) &&
-                        row_aligned(dn, lddn, d->dtype) && row_aligned(dx, d->C, d->dtype) && row_aligned(dh, d->C, d->dtype) && d->C % 8 == 0;
+                        row_aligned(dn, lddn, d->dtype) && row_aligned(dx, d->C, d->dtype) && row_aligned(dh, d->C, d->dtype) && d->C % 8 == 0 &&
+                        par_aligned({gate, scale, post_w, post_b, pre_w});
         with_layout(d->C, [&](auto lpr, auto vpl) {
             constexpr int L = decltype(lpr)::value, V = decltype(vpl)::value;
-            RDFC_DISPATCH(d->dtype, if (al) norm_residual_bwd_kernel<T, L, V, true><<<grid, NT, 0, (hipStream_t)stream>>>(p);
-                          else norm_residual_bwd_kernel<T, L, V, false><<<grid, NT, 0, (hipStream_t)stream>>>(p));
+            RDFC_DISPATCH(d->dtype, if (al) norm_residual_bwd_kernel<T, L, V, true><<<grid, threads_of(L), 0, (hipStream_t)stream>>>(p);
+                          else norm_residual_bwd_kernel<T, L, V, false><<<grid, threads_of(L), 0, (hipStream_t)stream>>>(p));
         });
         RDFC_LAUNCH_CHECK("rdfc_norm_residual_backward");
     }
@@ -611,7 +659,7 @@ extern "C" int rdfc_norm_residual_backward(const rdfc_norm_residual_desc *d, con
         double *sums = reinterpret_cast<double *>(scratch + k.partial);         // (8-byte aligned: partial is a multiple of 4)
         if (!empty)
             norm_residual_sum_kernel<<<dim3(cdiv(4 * d->C, SUM_COLS), samples, k.slices), SUM_COLS * SUM_ROWS, 0, (hipStream_t)stream>>>(scratch, sums, 4 * d->C, k.nchunk);
-        norm_residual_grads_kernel<<<cdiv(d->C, 64), 64, 0, (hipStream_t)stream>>>(p, o, sums, samples, k.slices);
+        norm_residual_grads_kernel<<<cdiv(d->C, 64), 512, 0, (hipStream_t)stream>>>(p, o, sums, samples, k.slices);
         RDFC_LAUNCH_CHECK("rdfc_norm_residual_backward (columns)");
     }
     return 0;

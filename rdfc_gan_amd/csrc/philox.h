@@ -46,8 +46,8 @@ __device__ __forceinline__ u32x4 philox(unsigned long long q, unsigned long long
 }
 __device__ __forceinline__ unsigned word16(const u32x4 &w, int i) { return i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu; }
 
-// bit i of the result: element e0 + i is kept (i = 0 .. 7; two calls where e0 is not a multiple of 8)
-__device__ __forceinline__ unsigned keep8(unsigned long long e0, unsigned threshold, unsigned long long seed, unsigned long long offset) {
+// bit i of the result: element e0 + i is kept (i = 0 .. 7).  WHOLE: e0 is a multiple of 8; else two calls where it is not
+template <bool WHOLE = false> __device__ __forceinline__ unsigned keep8(unsigned long long e0, unsigned threshold, unsigned long long seed, unsigned long long offset) {
     auto bits = [&](unsigned long long q) {
         const u32x4 w = philox(q, seed, offset);
         unsigned m = 0;
@@ -55,8 +55,10 @@ __device__ __forceinline__ unsigned keep8(unsigned long long e0, unsigned thresh
         for (int i = 0; i < 8; ++i) m |= (word16(w, i) >= threshold ? 1u : 0u) << i;
         return m;
     };
-    const int s = (int)(e0 & 7);
     unsigned m = bits(e0 >> 3);
-    if (s) m = (m | bits((e0 >> 3) + 1) << 8) >> s;
+    if constexpr (!WHOLE) {
+        const int s = (int)(e0 & 7);
+        if (s) m = (m | bits((e0 >> 3) + 1) << 8) >> s;
+    }
     return m;
 }

@@ -19,10 +19,10 @@ struct GLArgs {
     const void *x, *wg, *wu, *dz;
     const float *bg, *bu;
     void *z, *D, *dx;
-    float *partial;                  // BWD: bias sums [row block][2 Fp];  DW: [split][2 Fp][K]
+    float *partial;                  // BWD: bias sums [row block][2 Fp];  DW: [split][2 Fp][K];  DX: [split][M][K], or null: dx is written
     int64_t M;
     int K, Kv, F, Fp, ldx, ldwg, ldwu, lddz, act;   // Kv: K in whole 16-byte vectors (what lies between is zero)
-    int64_t split_rows;              // DW: pixels per split
+    int64_t split_rows;              // contraction per split: pixels (DW), columns of D (DX)
 };
 
 // ---- activation of the gate and its derivative ---------------------------------------------------------------------------------
@@ -150,16 +150,22 @@ __global__ __launch_bounds__(NT, 2) void gated_dma_kernel(GLArgs p, int tiles_p,
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char *)smem;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wp = wave >> 1, wq = wave & 1;
-    // workgroups are dealt to the 8 XCDs in turn: the P tiles of a Q tile (the pixels) follow each other on one XCD and share its L2
-    int64_t tq;
-    int tp;
-    {
-        const int64_t id = blockIdx.x, local = id >> 3;
-        tq = (local / tiles_p) * 8 + (id & 7);
-        tp = (int)(local % tiles_p);
-        if (tq >= tiles_q) return;
-    }
+    // Workgroups are dealt to the 8 XCDs in turn.  Each XCD takes one eighth of the tiles, P tiles of a Q tile (the pixels) side by side: they
+    // share what its L2 holds of the pixels, and every XCD has the same number of them whatever the sizes.
+    const int64_t tiles = tiles_q * tiles_p, per = (tiles + 7) >> 3, local = blockIdx.x >> 3, index = (blockIdx.x & 7) * per + local;
+    if (local >= per || index >= tiles) return;
+    int64_t tq = index / tiles_p;
+    int tp = (int)(index - tq * tiles_p);
     int64_t kbeg = 0, kend = MODE == DX ? 2 * p.Fp : p.Kv;
+    int split = 0;
+    if constexpr (MODE == DX) {
+        // (the splits of a tile side by side)
+        const int splits = (int)((kend + p.split_rows - 1) / p.split_rows);
+        split = tp % splits;
+        tp /= splits;
+        kbeg = split * p.split_rows;
+        kend = min(kbeg + p.split_rows, kend);
+    }
     int64_t q0 = tq * BQ;
     if constexpr (MODE == DW) {
         // (the pixels are contracted: tq numbers the splits, tp the output tiles)
@@ -444,6 +450,19 @@ __global__ __launch_bounds__(NT, 2) void gated_dma_kernel(GLArgs p, int tiles_p,
         });
     } else if constexpr (MODE == DX) {
         const int kw = p0 + wp * WTP;
+        if (p.partial != nullptr) {
+#pragma unroll
+            for (int j = 0; j < QT; ++j) {
+                const int64_t m = q0 + wq * WTQ + 16 * j + l16;
+                if (m >= p.M) continue;
+                float *out = p.partial + ((size_t)split * p.M + m) * p.K;
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    for (int r = 0; r < 4; ++r)
+                        if (kw + 16 * i + q4 + r < p.K) out[kw + 16 * i + q4 + r] = acc[i][j][r];
+            }
+            return;
+        }
         const bool vec = p.K * ES % 16 == 0 && (reinterpret_cast<size_t>(p.dx) & 15) == 0;
 #pragma unroll
         for (int j = 0; j < QT; ++j) {
@@ -474,15 +493,15 @@ __global__ __launch_bounds__(NT, 2) void gated_dma_kernel(GLArgs p, int tiles_p,
     }
 }
 
-// out[kind][f][k] = sum over parts of partial[part][kind * Fp + f][k], in the order of the parts
-template <typename TO> __global__ __launch_bounds__(NT) void gated_join_kernel(const float *__restrict__ partial, int parts, int F, int Fp, int K, TO *o0, TO *o1) {
-    const size_t n = (size_t)F * K, i = (size_t)blockIdx.x * NT + threadIdx.x;
-    if (i >= n) return;
-    const size_t step = (size_t)2 * Fp * K, src = (size_t)blockIdx.y * Fp * K + i;
+// o0 (o1: the second half of a part) [n] = sum over the parts of partial[part][step], in the order of the parts, in f64
+template <typename TO> __global__ __launch_bounds__(NT) void gated_join_kernel(const float *__restrict__ partial, int parts, size_t n, size_t step, TO *o0, TO *o1) {
+    const size_t i = (size_t)blockIdx.x * NT + threadIdx.x;
     TO *o = blockIdx.y ? o1 : o0;
-    if (o == nullptr) return;
+    if (i >= n || o == nullptr) return;
+    const float *src = partial + i + (blockIdx.y ? step / 2 : 0);
     double s = 0.;
-    for (int k = 0; k < parts; ++k) s += (double)partial[k * step + src];
+#pragma unroll 8
+    for (int k = 0; k < parts; ++k) s += (double)src[k * step];
     Elem<TO>::st(o + i, (float)s);
 }
 
@@ -553,14 +572,16 @@ int pack(const rdfc_gated_desc *d, const Packs &q, GLArgs &p, void *scratch, hip
 struct Tile {
     int wtp, wtq;
 };
-// the largest wave tile that still gives every CU work: `of(tile)` -> workgroups
-template <typename F> Tile tile_of(F &&of) {
-    if (of(Tile{128, 64}) >= 384) return Tile{128, 64};
-    if (of(Tile{64, 64}) >= 256) return Tile{64, 64};
-    return Tile{32, 32};
+// Wave tile from the workgroups that 64 x 64 gives: below one per CU the chip is better filled by 32 x 32 (288 x 512 -> 1365, f16: 8.3 us against
+// 11.3; f32 dx of 2280 x 512: 126 against 205).  128 x 64 moves a quarter fewer bytes through the L1 per product, but leaves two
+// workgroups on a CU where 64 x 64 has three, and the backward kernel spills: it pays in the forward pass alone, from
+// K = 768 (34656 x 1024 -> 1024, f16: 159 us against 179; at K = 256 63 against 60, at 512 56 against 56).
+template <typename F> Tile tile_of(F &&of, bool wide = false) {
+    if (wide && of(Tile{128, 64}) >= 384) return Tile{128, 64};
+    return of(Tile{64, 64}) >= 256 ? Tile{64, 64} : Tile{32, 32};
 }
 template <int MODE> int launch_dma(const GLArgs &p, int dtype, Tile t, int tiles_p, int64_t tiles_q, hipStream_t st, const char *name) {
-    const int64_t grid = (tiles_q + 7) / 8 * 8 * tiles_p;
+    const int64_t grid = (tiles_q * tiles_p + 7) / 8 * 8;
     RDFC_REQUIRE(grid < (1ll << 31), "%s: %lld workgroups are too many", name, (long long)grid);
     auto go = [&](auto dt, auto wtp, auto wtq) {
         constexpr int WTP = decltype(wtp)::value, WTQ = decltype(wtq)::value, LDS = 3 * (2 * WTP + 2 * WTQ) * 64;
@@ -574,8 +595,13 @@ template <int MODE> int launch_dma(const GLArgs &p, int dtype, Tile t, int tiles
         kernel<<<dim3((unsigned)grid), NT, LDS, st>>>(p, tiles_p, tiles_q);
     };
     auto size = [&](auto dt) {
-        if (t.wtp == 128) go(dt, std::integral_constant<int, 128>{}, std::integral_constant<int, 64>{});
-        else if (t.wtp == 64) go(dt, std::integral_constant<int, 64>{}, std::integral_constant<int, 64>{});
+        if constexpr (MODE == FWD) {
+            if (t.wtp == 128) {
+                go(dt, std::integral_constant<int, 128>{}, std::integral_constant<int, 64>{});
+                return;
+            }
+        }
+        if (t.wtp == 64) go(dt, std::integral_constant<int, 64>{}, std::integral_constant<int, 64>{});
         else go(dt, std::integral_constant<int, 32>{}, std::integral_constant<int, 32>{});
     };
     if (dtype == RDFC_BF16) size(std::integral_constant<int, RDFC_BF16>{});
@@ -586,10 +612,10 @@ template <int MODE> int launch_dma(const GLArgs &p, int dtype, Tile t, int tiles
 }
 
 struct Plan {
-    int Fp, row_blocks, splits;
+    int Fp, row_blocks, splits, dx_splits;
     Tile gated, dx, dw;
-    int64_t split_rows;
-    size_t d_bytes, bias_floats, w_floats;
+    int64_t split_rows, dx_cols;
+    size_t d_bytes, bias_floats, w_floats, dx_floats;
 };
 Plan plan_of(const rdfc_gated_desc *d) {
     Plan p;
@@ -597,10 +623,19 @@ Plan plan_of(const rdfc_gated_desc *d) {
     p.gated = tile_of([&](Tile t) { return cdiv(p.Fp, t.wtp) * (int64_t)cdiv(d->M, 2 * t.wtq); });
     p.dx = tile_of([&](Tile t) { return cdiv(d->K, 2 * t.wtp) * (int64_t)cdiv(d->M, 2 * t.wtq); });
     p.row_blocks = cdiv(d->M, 64);                               // (of the smallest tile: an upper bound)
+    // dx: the contraction (2 Fp) is split where its tiles would leave CUs idle, f32 parts joined afterwards (2280 x 512, f32: 126 -> %DX% us)
+    const int64_t dx_tiles = (int64_t)cdiv(d->K, 2 * p.dx.wtp) * cdiv(d->M, 2 * p.dx.wtq);
+    int64_t ds = dx_tiles > 0 ? 512 / dx_tiles : 1;
+    const int64_t ds_most = 2 * p.Fp / 256;
+    ds = ds > 8 ? 8 : ds;
+    ds = ds > ds_most ? ds_most : ds;
+    ds = ds < 1 ? 1 : ds;
+    p.dx_cols = (2 * p.Fp / ds + 31) / 32 * 32;
+    p.dx_splits = (int)((2 * p.Fp + p.dx_cols - 1) / p.dx_cols);
     const int64_t most = (d->M + 255) / 256;
     p.dw = tile_of([&](Tile t) { return cdiv(d->K, 2 * t.wtp) * (int64_t)cdiv(2 * p.Fp, 2 * t.wtq) * (most < 32 ? most : 32); });
     const int64_t tiles = (int64_t)cdiv(d->K, 2 * p.dw.wtp) * cdiv(2 * p.Fp, 2 * p.dw.wtq);
-    int64_t s = 512 / tiles;
+    int64_t s = 768 / tiles;                                     // three workgroups a CU
     s = s > most ? most : s;
     s = s < 1 ? 1 : s;
     p.split_rows = ((d->M + s - 1) / s + 31) / 32 * 32;
@@ -608,7 +643,8 @@ Plan plan_of(const rdfc_gated_desc *d) {
     p.splits = (int)((d->M + p.split_rows - 1) / p.split_rows);
     p.d_bytes = ((size_t)d->M * 2 * p.Fp * (d->dtype == RDFC_F32 ? 4 : 2) + 255) / 256 * 256;
     p.bias_floats = ((size_t)p.row_blocks * 2 * p.Fp + 63) / 64 * 64;
-    p.w_floats = (size_t)p.splits * 2 * p.Fp * d->K;
+    p.w_floats = ((size_t)p.splits * 2 * p.Fp * d->K + 63) / 64 * 64;
+    p.dx_floats = p.dx_splits > 1 ? (size_t)p.dx_splits * d->M * d->K : 0;
     return p;
 }
 int check(const rdfc_gated_desc *d, const char *name) {
@@ -653,7 +689,7 @@ extern "C" int rdfc_gated_linear(const rdfc_gated_desc *d, const void *x, const 
     GLArgs p = args(d, x, wg, wu, bg, bu);
     if (pack(d, k, p, scratch, (hipStream_t)stream, "rdfc_gated_linear (pack)")) return 2;
     p.z = z;
-    const Tile t = tile_of([&](Tile t) { return cdiv(d->F, t.wtp) * (int64_t)cdiv(d->M, 2 * t.wtq); });
+    const Tile t = tile_of([&](Tile t) { return cdiv(d->F, t.wtp) * (int64_t)cdiv(d->M, 2 * t.wtq); }, d->K >= 768);
     return launch_dma<FWD>(p, d->dtype, t, cdiv(d->F, t.wtp), cdiv(d->M, 2 * t.wtq), (hipStream_t)stream, "rdfc_gated_linear");
 }
 
@@ -662,7 +698,7 @@ extern "C" size_t rdfc_gated_linear_scratch_bytes(const rdfc_gated_desc *d, cons
     const size_t k = packs_of(d, x, wg, wu).bytes();
     if (!backward) return k;
     const Plan q = plan_of(d);
-    return k + q.d_bytes + 4 * (q.bias_floats + q.w_floats);
+    return k + q.d_bytes + 4 * (q.bias_floats + (q.w_floats > q.dx_floats ? q.w_floats : q.dx_floats));
 }
 
 extern "C" int rdfc_gated_linear_backward(const rdfc_gated_desc *d, const void *x, const void *wg, const void *wu, const float *bg, const float *bu,
@@ -689,7 +725,14 @@ extern "C" int rdfc_gated_linear_backward(const rdfc_gated_desc *d, const void *
         if (launch_dma<BWD>(p, d->dtype, q.gated, cdiv(q.Fp, q.gated.wtp), row_blocks, st, "rdfc_gated_linear_backward")) return 2;
         if (dx) {
             p.dx = dx;
-            if (launch_dma<DX>(p, d->dtype, q.dx, cdiv(d->K, 2 * q.dx.wtp), cdiv(d->M, 2 * q.dx.wtq), st, "rdfc_gated_linear_backward (input)")) return 2;
+            p.partial = q.dx_splits > 1 ? w : nullptr;           // (the weight gradients' parts follow in the same memory)
+            p.split_rows = q.dx_cols;
+            if (launch_dma<DX>(p, d->dtype, q.dx, cdiv(d->K, 2 * q.dx.wtp) * q.dx_splits, cdiv(d->M, 2 * q.dx.wtq), st, "rdfc_gated_linear_backward (input)")) return 2;
+            if (q.dx_splits > 1) {
+                const size_t n = (size_t)d->M * d->K;
+                RDFC_DISPATCH(d->dtype, (gated_join_kernel<T><<<dim3((unsigned)((n + NT - 1) / NT), 1), NT, 0, st>>>(w, q.dx_splits, n, n, (T *)dx, nullptr)));
+                RDFC_LAUNCH_CHECK("rdfc_gated_linear_backward (input join)");
+            }
         }
         if (dwg || dwu) {
             p.partial = w;
@@ -705,7 +748,7 @@ extern "C" int rdfc_gated_linear_backward(const rdfc_gated_desc *d, const void *
     }
     if (dwg || dwu) {
         const dim3 grid((unsigned)(((size_t)d->F * d->K + NT - 1) / NT), 2);
-        RDFC_DISPATCH(dw_dtype, (gated_join_kernel<T><<<grid, NT, 0, st>>>(w, d->M > 0 ? q.splits : 0, d->F, q.Fp, d->K, (T *)dwg, (T *)dwu)));
+        RDFC_DISPATCH(dw_dtype, (gated_join_kernel<T><<<grid, NT, 0, st>>>(w, d->M > 0 ? q.splits : 0, (size_t)d->F * d->K, (size_t)2 * q.Fp * d->K, (T *)dwg, (T *)dwu)));
         RDFC_LAUNCH_CHECK("rdfc_gated_linear_backward (join)");
     }
     return 0;

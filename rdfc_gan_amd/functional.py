@@ -1090,6 +1090,8 @@ def _check_param(t, what, shape, device):
     """a parameter vector: f32 (cast where it is not), dense"""
     if t is None:
         return None
+    if t.shape == shape and t.dtype == torch.float32 and t.device == device and t.is_contiguous():
+        return t
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f'{what}: shape {tuple(t.shape)}, expected {tuple(shape)}')
     if t.device != device or not t.is_floating_point():
@@ -1105,7 +1107,9 @@ class _Dropout(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return _Dropout.apply(dy, *ctx.args), None, None, None, None
+        if dy.requires_grad and torch.is_grad_enabled():              # (a second derivative is asked for)
+            return _Dropout.apply(dy, *ctx.args), None, None, None, None
+        return hip.dropout(hip.as_pm(dy), *ctx.args), None, None, None, None
 
 
 def dropout(x, p, training=True, rng=None):

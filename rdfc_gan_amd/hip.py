@@ -1058,9 +1058,15 @@ class GatedDesc(C.Structure):
 GATE_ACT = dict(relu=1, sigmoid=4, silu=16, gelu=17)
 
 
+_entry = {}
+
+
 def _call(name, t, *args):
     """one entry point on t's device and that device's current stream (whatever the current device is)"""
-    fn, dev = getattr(lib(), name), t.device.index
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(lib(), name)
+    dev = t.get_device()
     if dev == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
@@ -1068,6 +1074,11 @@ def _call(name, t, *args):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     if rc != 0:
         _chk(rc, name)
+
+
+def _a(t):
+    """address of a tensor that has been checked already"""
+    return None if t is None else t.data_ptr()
 
 
 def as_pm(t):
@@ -1082,13 +1093,13 @@ def dropout(x, threshold, seed, offset, key=None):
     N, H, W, Cc = x.shape
     y = torch.empty(N, H, W, Cc, dtype=x.dtype, device=x.device)
     if y.numel():
-        _call('rdfc_dropout', x, _p(x), _p(y), N * H * W, Cc, ld(x), Cc, dt(x), threshold, seed, offset, _p(key))
+        _call('rdfc_dropout', x, _a(x), _a(y), N * H * W, Cc, ld(x), Cc, dt(x), threshold, seed, offset, _a(key))
     return y
 
 
 def dropout_draw(state):
     key = torch.empty(2, dtype=torch.int64, device=state.device)
-    _call('rdfc_dropout_draw', state, _p(state), _p(key))
+    _call('rdfc_dropout_draw', state, _a(state), _a(key))
     return key
 
 
@@ -1104,7 +1115,7 @@ def norm_residual(x, h, gate, scale, post, pre, layer, eps, threshold, seed, off
     if x.numel():
         pw, pb = post or (None, None)
         qw, qb = pre or (None, None)
-        _call('rdfc_norm_residual', x, C.byref(d), _p(x), _p(h), _p(gate), _p(scale), _p(pw), _p(pb), _p(qw), _p(qb), _p(key), _p(y), _p(n), _p(stats))
+        _call('rdfc_norm_residual', x, C.byref(d), _a(x), _a(h), _a(gate), _a(scale), _a(pw), _a(pb), _a(qw), _a(qb), _a(key), _a(y), _a(n), _a(stats))
     return d, y, n, stats
 
 
@@ -1115,17 +1126,20 @@ def norm_residual_backward(d, x, h, gate, scale, post, pre, key, stats, dy, dn, 
     qw = pre[0] if pre else None
     dx = torch.empty(N, H, W, Cc, dtype=x.dtype, device=x.device)
     dh = torch.empty_like(dx) if h is not None else None
-    cols = [torch.empty((N, Cc) if i == 0 else (Cc,), dtype=torch.float32, device=x.device) if w else None for i, w in enumerate(want)]
-    scratch = None
+    cols, scratch = [None] * 6, None
     if any(want):
+        # (the small gradients are slices of one allocation)
+        sizes = [(N if i == 0 else 1) * Cc for i, w in enumerate(want) if w]
+        flat = iter(torch.empty(sum(sizes), dtype=torch.float32, device=x.device).split(sizes))
+        cols = [(next(flat).view(N, Cc) if i == 0 else next(flat)) if w else None for i, w in enumerate(want)]
         scratch = torch.empty(lib().rdfc_norm_residual_scratch_floats(C.byref(d), int(gate is not None)), dtype=torch.float32, device=x.device)
-    _call('rdfc_norm_residual_backward', x, C.byref(d), _p(x), _p(h), _p(gate), _p(scale), _p(pw), _p(pb), _p(qw), _p(key), _p(stats), _p(dy),
-          ld(dy) if dy is not None else Cc, _p(dn), ld(dn) if dn is not None else Cc, _p(dx), _p(dh), _p(scratch), *map(_p, cols))
+    _call('rdfc_norm_residual_backward', x, C.byref(d), _a(x), _a(h), _a(gate), _a(scale), _a(pw), _a(pb), _a(qw), _a(key), _a(stats), _a(dy),
+          ld(dy) if dy is not None else Cc, _a(dn), ld(dn) if dn is not None else Cc, _a(dx), _a(dh), _a(scratch), *map(_a, cols))
     return (dx, dh, *cols)
 
 
 def _gated_scratch(d, x, wg, wu, backward):
-    n = lib().rdfc_gated_linear_scratch_bytes(C.byref(d), _p(x), _p(wg), _p(wu), backward)
+    n = lib().rdfc_gated_linear_scratch_bytes(C.byref(d), _a(x), _a(wg), _a(wu), backward)
     return torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
 
 
@@ -1137,7 +1151,7 @@ def gated_linear(x, wg, wu, bg, bu, act):
     z = torch.empty(N, H, W, F, dtype=x.dtype, device=x.device)
     if z.numel():
         scratch = _gated_scratch(d, x, wg, wu, 0)
-        _call('rdfc_gated_linear', x, C.byref(d), _p(x), _p(wg), _p(wu), _p(bg), _p(bu), _p(scratch), _p(z))
+        _call('rdfc_gated_linear', x, C.byref(d), _a(x), _a(wg), _a(wu), _a(bg), _a(bu), _a(scratch), _a(z))
     return d, z
 
 
@@ -1149,6 +1163,6 @@ def gated_linear_backward(d, x, wg, wu, bg, bu, dz, want_dx, dw_dtype, want_bias
     dwg, dwu = (torch.empty(F, K, dtype=dw_dtype, device=x.device) for _ in range(2)) if dw_dtype is not None else (None, None)
     dbg, dbu = (torch.empty(F, dtype=torch.float32, device=x.device) for _ in range(2)) if want_bias else (None, None)
     scratch = _gated_scratch(d, x, wg, wu, 1)
-    _call('rdfc_gated_linear_backward', x, C.byref(d), _p(x), _p(wg), _p(wu), _p(bg), _p(bu), _p(dz), ld(dz), _p(scratch), _p(dx), _p(dwg), _p(dwu),
-          F32 if dw_dtype == torch.float32 else dt(x), _p(dbg), _p(dbu))
+    _call('rdfc_gated_linear_backward', x, C.byref(d), _a(x), _a(wg), _a(wu), _a(bg), _a(bu), _a(dz), ld(dz), _a(scratch), _a(dx), _a(dwg), _a(dwu),
+          F32 if dw_dtype == torch.float32 else dt(x), _a(dbg), _a(dbu))
     return dx, dwg, dwu, dbg, dbu

@@ -583,15 +583,16 @@ typedef struct rdfc_gated_desc {
     int32_t K, F, ldx, ldwg, ldwu, dtype, act;
 } rdfc_gated_desc;
 /* bytes of scratch (256-byte aligned) that a forward or backward call with these operands needs; the pointers' alignment counts, not what
- * they point to: rows that are not whole 16-byte vectors are copied first.  0: scratch may be NULL. */
+ * they point to: rows that are not whole 16-byte vectors are copied first.  0: scratch may be NULL.
+ * pre: f32 maps only, [M][2 Fp] with Fp = F rounded up to 32: g and u for the backward pass; NULL without one. */
 size_t rdfc_gated_linear_scratch_bytes(const rdfc_gated_desc *d, const void *x, const void *wg, const void *wu, int backward);
 int rdfc_gated_linear(const rdfc_gated_desc *d, const void *x, const void *wg, const void *wu, const float *bg, const float *bu, void *scratch,
-                      void *z, void *stream);
+                      void *z, float *pre, void *stream);
 /* dz [M][F] (lddz) -> dx dense [M][K], dwg, dwu dense [F][K] (dw_dtype: RDFC_F32 or the map's type), dbg, dbu f32 [F]; each may be NULL.
- * g and u are computed again; dg and du are rounded to the map's type for the two products, the bias gradients
- * are summed before that.  Sums have a fixed order. */
-int rdfc_gated_linear_backward(const rdfc_gated_desc *d, const void *x, const void *wg, const void *wu, const float *bg, const float *bu, const void *dz,
-                               int lddz, void *scratch, void *dx, void *dwg, void *dwu, int dw_dtype, float *dbg, float *dbu, void *stream);
+ * 16-bit maps: g and u are computed again (pre = NULL); dg and du are rounded to the map's type for the two products, the bias gradients
+ * are summed before that.  f32 maps: pre as the forward call wrote it.  Sums have a fixed order. */
+int rdfc_gated_linear_backward(const rdfc_gated_desc *d, const void *x, const void *wg, const void *wu, const float *bg, const float *bu, const float *pre,
+                               const void *dz, int lddz, void *scratch, void *dx, void *dwg, void *dwu, int dw_dtype, float *dbg, float *dbu, void *stream);
 
 #ifdef __cplusplus
 }

@@ -4,9 +4,12 @@
 //
 // Forward: one product whose weight rows alternate 16 of Wg with 16 of Wu, so that a lane's accumulators hold g and u of the same
 // elements and the activation and the product happen in registers: g and u never reach memory.
-// Backward: the same product again, with dz in the epilogue: dg = dz u act'(g) and du = dz act(g), side by side in one map
+// Backward, 16-bit maps: the same product again, with dz in the epilogue: dg = dz u act'(g) and du = dz act(g), side by side in one map
 // D [M][2 Fp] (Fp = F rounded up to 32, the columns between zero), with the bias gradients' partial sums in f32 beside the rounding to
-// the map's type.  Then dx = D [Wg; Wu] and [dWg; dWu] = D^T x, the latter split over the pixels and joined in a fixed order.
+// the map's type.  Keeping g and u instead would round them to 16 bits, and their traffic costs more than the product up to K of about 400
+// (34656 x 256 -> 1024: 142 MB written and 213 read, 70 us at the rate of a copy, against 36 GFLOP).  f32 maps keep them: nothing is rounded, and the
+// product costs fifteen times as much (2280 x 512 -> 1365: 74 us against 14 for an elementwise pass).
+// Then dx = D [Wg; Wu] and [dWg; dWu] = D^T x, the latter split over the pixels and joined in a fixed order.
 #include "common.h"
 
 namespace {
@@ -19,6 +22,7 @@ struct GLArgs {
     const void *x, *wg, *wu, *dz;
     const float *bg, *bu;
     void *z, *D, *dx;
+    float *pre;                      // f32 maps: g and u, [M][2 Fp], written by the forward pass for the backward one (or null)
     float *partial;                  // BWD: bias sums [row block][2 Fp];  DW: [split][2 Fp][K];  DX: [split][M][K], or null: dx is written
     int64_t M;
     int K, Kv, F, Fp, ldx, ldwg, ldwu, lddz, act;   // Kv: K in whole 16-byte vectors (what lies between is zero)
@@ -364,6 +368,19 @@ __global__ __launch_bounds__(NT, 2) void gated_dma_kernel(GLArgs p, int tiles_p,
                 const bool vec = p.F * ES % 16 == 0 && (reinterpret_cast<size_t>(p.z) & 15) == 0;
 #pragma unroll
                 for (int j = 0; j < QT; ++j) {
+                    if constexpr (ES == 4) {
+                        if (p.pre != nullptr) {
+#pragma unroll
+                            for (int kind = 0; kind < 2; ++kind) {
+#pragma unroll
+                                for (int i = 0; i < MT / 2; ++i) {
+                                    const float v[4] = {acc[2 * i + kind][j][0], acc[2 * i + kind][j][1], acc[2 * i + kind][j][2], acc[2 * i + kind][j][3]};
+                                    put(16 * i + q4, v);
+                                }
+                                flush(p.pre + kind * p.Fp + fw, q0 + wq * WTQ + 16 * j, 2 * p.Fp, p.Fp - fw, true);
+                            }
+                        }
+                    }
 #pragma unroll
                     for (int i = 0; i < MT / 2; ++i) {
                         float v[4];
@@ -493,6 +510,53 @@ __global__ __launch_bounds__(NT, 2) void gated_dma_kernel(GLArgs p, int tiles_p,
     }
 }
 
+// D and the bias sums of ACT_ROWS pixels from the kept g and u (f32): 64 lanes of 4 features x 4 row lanes
+constexpr int ACT_ROWS = 64;
+__global__ __launch_bounds__(NT) void gated_act_kernel(GLArgs p) {
+    __shared__ float red[4][2][256];
+    const int cl = threadIdx.x & 63, rl = threadIdx.x >> 6, f = (blockIdx.y * 64 + cl) * 4;
+    const int64_t m0 = (int64_t)blockIdx.x * ACT_ROWS, m1 = min(m0 + ACT_ROWS, p.M);
+    float sg[4] = {0.f, 0.f, 0.f, 0.f}, su[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool vec = p.lddz % 4 == 0 && (reinterpret_cast<size_t>(p.dz) & 15) == 0;
+    if (f < p.Fp) {
+        with_gate(p.act, [&](auto act) {
+#pragma unroll 4
+            for (int64_t m = m0 + rl; m < m1; m += 4) {
+                const f32x4 g = *reinterpret_cast<const f32x4 *>(p.pre + m * 2 * p.Fp + f), u = *reinterpret_cast<const f32x4 *>(p.pre + m * 2 * p.Fp + p.Fp + f);
+                const float *src = (const float *)p.dz + m * p.lddz + f;
+                f32x4 dz = {0.f, 0.f, 0.f, 0.f}, dg, du;
+                if (vec && f + 3 < p.F) dz = *reinterpret_cast<const f32x4 *>(src);
+                else
+                    for (int r = 0; r < 4; ++r)
+                        if (f + r < p.F) dz[r] = src[r];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float a, da;
+                    gate_act<decltype(act)::value, true>(g[r], a, da);
+                    dg[r] = f + r < p.F ? dz[r] * u[r] * da : 0.f;
+                    du[r] = f + r < p.F ? dz[r] * a : 0.f;
+                    sg[r] += dg[r];
+                    su[r] += du[r];
+                }
+                *reinterpret_cast<f32x4 *>((float *)p.D + m * 2 * p.Fp + f) = dg;
+                *reinterpret_cast<f32x4 *>((float *)p.D + m * 2 * p.Fp + p.Fp + f) = du;
+            }
+        });
+    }
+    if (p.partial == nullptr) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        red[rl][0][cl * 4 + r] = sg[r];
+        red[rl][1][cl * 4 + r] = su[r];
+    }
+    __syncthreads();
+    const int c = blockIdx.y * 256 + threadIdx.x;
+    if (c >= p.Fp) return;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        p.partial[(size_t)blockIdx.x * 2 * p.Fp + k * p.Fp + c] = (red[0][k][threadIdx.x] + red[1][k][threadIdx.x]) + (red[2][k][threadIdx.x] + red[3][k][threadIdx.x]);
+}
+
 // o0 (o1: the second half of a part) [n] = sum over the parts of partial[part][step], in the order of the parts, in f64
 template <typename TO> __global__ __launch_bounds__(NT) void gated_join_kernel(const float *__restrict__ partial, int parts, size_t n, size_t step, TO *o0, TO *o1) {
     const size_t i = (size_t)blockIdx.x * NT + threadIdx.x;
@@ -606,7 +670,7 @@ template <int MODE> int launch_dma(const GLArgs &p, int dtype, Tile t, int tiles
     };
     if (dtype == RDFC_BF16) size(std::integral_constant<int, RDFC_BF16>{});
     else if (dtype == RDFC_F16) size(std::integral_constant<int, RDFC_F16>{});
-    else size(std::integral_constant<int, RDFC_F32>{});
+    else if constexpr (MODE != BWD) size(std::integral_constant<int, RDFC_F32>{});
     RDFC_LAUNCH_CHECK(name);
     return 0;
 }
@@ -623,9 +687,9 @@ Plan plan_of(const rdfc_gated_desc *d) {
     p.gated = tile_of([&](Tile t) { return cdiv(p.Fp, t.wtp) * (int64_t)cdiv(d->M, 2 * t.wtq); });
     p.dx = tile_of([&](Tile t) { return cdiv(d->K, 2 * t.wtp) * (int64_t)cdiv(d->M, 2 * t.wtq); });
     p.row_blocks = cdiv(d->M, 64);                               // (of the smallest tile: an upper bound)
-    // dx: the contraction (2 Fp) is split where its tiles would leave CUs idle, f32 parts joined afterwards (2280 x 512, f32: 126 -> %DX% us)
+    // dx: the contraction (2 Fp) is split where its tiles would leave CUs idle, f32 parts joined afterwards (2280 x 512, f32: 126 -> 91 us)
     const int64_t dx_tiles = (int64_t)cdiv(d->K, 2 * p.dx.wtp) * cdiv(d->M, 2 * p.dx.wtq);
-    int64_t ds = dx_tiles > 0 ? 512 / dx_tiles : 1;
+    int64_t ds = dx_tiles > 0 && p.dx.wtp == 32 ? 1024 / dx_tiles : 1;
     const int64_t ds_most = 2 * p.Fp / 256;
     ds = ds > 8 ? 8 : ds;
     ds = ds > ds_most ? ds_most : ds;
@@ -635,7 +699,9 @@ Plan plan_of(const rdfc_gated_desc *d) {
     const int64_t most = (d->M + 255) / 256;
     p.dw = tile_of([&](Tile t) { return cdiv(d->K, 2 * t.wtp) * (int64_t)cdiv(2 * p.Fp, 2 * t.wtq) * (most < 32 ? most : 32); });
     const int64_t tiles = (int64_t)cdiv(d->K, 2 * p.dw.wtp) * cdiv(2 * p.Fp, 2 * p.dw.wtq);
-    int64_t s = 768 / tiles;                                     // three workgroups a CU
+    // two workgroups a CU (f32: three, what fits).  More parts cost the 16-bit maps more in the join than they fill: 34656 x 256 -> 1024, f16,
+    // 512 / 768 workgroups: 60 / 69 us; f32 2280 x 512 -> 1365: 76 / 70
+    int64_t s = (d->dtype == RDFC_F32 ? 768 : 512) / tiles;
     s = s > most ? most : s;
     s = s < 1 ? 1 : s;
     p.split_rows = ((d->M + s - 1) / s + 31) / 32 * 32;
@@ -679,7 +745,7 @@ GLArgs args(const rdfc_gated_desc *d, const void *x, const void *wg, const void 
 }  // namespace
 
 extern "C" int rdfc_gated_linear(const rdfc_gated_desc *d, const void *x, const void *wg, const void *wu, const float *bg, const float *bu, void *scratch,
-                                 void *z, void *stream) {
+                                 void *z, float *pre, void *stream) {
     if (check(d, "rdfc_gated_linear")) return 1;
     if (d->M == 0) return 0;
     RDFC_REQUIRE(x && wg && wu && z, "rdfc_gated_linear: null pointer");
@@ -688,7 +754,9 @@ extern "C" int rdfc_gated_linear(const rdfc_gated_desc *d, const void *x, const 
     RDFC_REQUIRE(k.bytes() == 0 || scratch, "rdfc_gated_linear: these operands need scratch memory");
     GLArgs p = args(d, x, wg, wu, bg, bu);
     if (pack(d, k, p, scratch, (hipStream_t)stream, "rdfc_gated_linear (pack)")) return 2;
+    RDFC_REQUIRE(!pre || (d->dtype == RDFC_F32 && (reinterpret_cast<size_t>(pre) & 15) == 0), "rdfc_gated_linear: pre is kept for f32 maps, 16-byte aligned");
     p.z = z;
+    p.pre = pre;
     const Tile t = tile_of([&](Tile t) { return cdiv(d->F, t.wtp) * (int64_t)cdiv(d->M, 2 * t.wtq); }, d->K >= 768);
     return launch_dma<FWD>(p, d->dtype, t, cdiv(d->F, t.wtp), cdiv(d->M, 2 * t.wtq), (hipStream_t)stream, "rdfc_gated_linear");
 }
@@ -702,7 +770,7 @@ extern "C" size_t rdfc_gated_linear_scratch_bytes(const rdfc_gated_desc *d, cons
 }
 
 extern "C" int rdfc_gated_linear_backward(const rdfc_gated_desc *d, const void *x, const void *wg, const void *wu, const float *bg, const float *bu,
-                                          const void *dz, int lddz, void *scratch, void *dx, void *dwg, void *dwu, int dw_dtype, float *dbg, float *dbu,
+                                          const float *pre, const void *dz, int lddz, void *scratch, void *dx, void *dwg, void *dwu, int dw_dtype, float *dbg, float *dbu,
                                           void *stream) {
     if (check(d, "rdfc_gated_linear_backward")) return 1;
     RDFC_REQUIRE(lddz >= d->F, "rdfc_gated_linear_backward: lddz smaller than F");
@@ -720,9 +788,17 @@ extern "C" int rdfc_gated_linear_backward(const rdfc_gated_desc *d, const void *
     int row_blocks = 0;
     if (d->M > 0) {
         if (pack(d, k, p, scratch, st, "rdfc_gated_linear_backward (pack)")) return 2;
-        row_blocks = cdiv(d->M, 2 * q.gated.wtq);
         p.partial = dbg || dbu ? bias : nullptr;
-        if (launch_dma<BWD>(p, d->dtype, q.gated, cdiv(q.Fp, q.gated.wtp), row_blocks, st, "rdfc_gated_linear_backward")) return 2;
+        if (d->dtype == RDFC_F32) {
+            RDFC_REQUIRE(pre, "rdfc_gated_linear_backward: f32 maps need the forward pass's pre");
+            p.pre = const_cast<float *>(pre);
+            row_blocks = cdiv(d->M, ACT_ROWS);
+            gated_act_kernel<<<dim3(row_blocks, cdiv(q.Fp, 256)), NT, 0, st>>>(p);
+            RDFC_LAUNCH_CHECK("rdfc_gated_linear_backward (activation)");
+        } else {
+            row_blocks = cdiv(d->M, 2 * q.gated.wtq);
+            if (launch_dma<BWD>(p, d->dtype, q.gated, cdiv(q.Fp, q.gated.wtp), row_blocks, st, "rdfc_gated_linear_backward")) return 2;
+        }
         if (dx) {
             p.dx = dx;
             p.partial = q.dx_splits > 1 ? w : nullptr;           // (the weight gradients' parts follow in the same memory)

@@ -1210,18 +1210,18 @@ class _GatedLinear(torch.autograd.Function):
         x = hip.as_pm(x)
         ctx.dw_dtype = wg.dtype
         wg, wu = (_weight_rows(w, x.dtype) for w in (wg, wu))
-        d, z = hip.gated_linear(x, wg, wu, bg, bu, act)
-        ctx.save_for_backward(x, wg, wu, bg, bu)
+        d, z, pre = hip.gated_linear(x, wg, wu, bg, bu, act, want_pre=any(ctx.needs_input_grad))
+        ctx.save_for_backward(x, wg, wu, bg, bu, pre)
         ctx.desc = d
         return z
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dz):
-        x, wg, wu, bg, bu = ctx.saved_tensors
+        x, wg, wu, bg, bu, pre = ctx.saved_tensors
         need = ctx.needs_input_grad
         dz = hip.as_pm(dz if dz.dtype == x.dtype else dz.to(x.dtype))
-        grads = hip.gated_linear_backward(ctx.desc, x, wg, wu, bg, bu, dz, need[0], ctx.dw_dtype if need[1] or need[2] else None, need[3] or need[4])
+        grads = hip.gated_linear_backward(ctx.desc, x, wg, wu, bg, bu, pre, dz, need[0], ctx.dw_dtype if need[1] or need[2] else None, need[3] or need[4])
         return (*(g if n else None for g, n in zip(grads, need)), None)
 
 
@@ -1235,8 +1235,9 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act='silu'):
     """z = act(x w_gate^T + b_gate) * (x w_up^T + b_up) on a pixel-major map x [N, H, W, K] -> [N, H, W, F]: both projections, the activation
     and the product in one kernel.  w_gate, w_up [F, K] (or 1x1 convolution weights [F, K, 1, 1]) in the map's type, or f32 masters beside a
     16-bit map (cast in the call; their gradients are then f32); b_gate, b_up f32 [F], both or neither.  act: 'silu', 'gelu' (exact),
-    'sigmoid' or 'relu'.  The backward pass computes both projections again; in 16-bit maps their cotangents are rounded to the map's
-    type before the products with the weights and with x, as every block here stores its cotangents."""
+    'sigmoid' or 'relu'.  For the backward pass f32 maps keep both projections (2 F values a pixel); 16-bit
+    maps compute them again, and round their cotangents to the map's type before the products with the weights and with x, as every block
+    here stores its cotangents."""
     _check_map(x, 'gated_linear')
     if act not in hip.GATE_ACT:
         raise ValueError(f'act is one of {sorted(hip.GATE_ACT)}, got {act!r}')

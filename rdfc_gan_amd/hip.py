@@ -1143,19 +1143,20 @@ def _gated_scratch(d, x, wg, wu, backward):
     return torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
 
 
-def gated_linear(x, wg, wu, bg, bu, act):
-    """-> (descriptor, z); x pixel-major, weights [F, K] rows of the map's type"""
+def gated_linear(x, wg, wu, bg, bu, act, want_pre=False):
+    """-> (descriptor, z, pre); x pixel-major, weights [F, K] rows of the map's type; want_pre: a backward pass follows (f32 maps keep g and u)"""
     N, H, W, K = x.shape
     F = wg.shape[0]
     d = GatedDesc(N * H * W, K, F, ld(x), wg.stride(0) if F > 1 else K, wu.stride(0) if F > 1 else K, dt(x), GATE_ACT[act])
     z = torch.empty(N, H, W, F, dtype=x.dtype, device=x.device)
+    pre = torch.empty(N * H * W, 2 * ((F + 31) // 32 * 32), dtype=torch.float32, device=x.device) if want_pre and x.dtype == torch.float32 else None
     if z.numel():
         scratch = _gated_scratch(d, x, wg, wu, 0)
-        _call('rdfc_gated_linear', x, C.byref(d), _a(x), _a(wg), _a(wu), _a(bg), _a(bu), _a(scratch), _a(z))
-    return d, z
+        _call('rdfc_gated_linear', x, C.byref(d), _a(x), _a(wg), _a(wu), _a(bg), _a(bu), _a(scratch), _a(z), _a(pre))
+    return d, z, pre
 
 
-def gated_linear_backward(d, x, wg, wu, bg, bu, dz, want_dx, dw_dtype, want_bias):
+def gated_linear_backward(d, x, wg, wu, bg, bu, pre, dz, want_dx, dw_dtype, want_bias):
     """dw_dtype: None (no weight gradients), f32 or the map's type -> (dx, dwg, dwu, dbg, dbu)"""
     N, H, W, K = x.shape
     F = wg.shape[0]
@@ -1163,6 +1164,6 @@ def gated_linear_backward(d, x, wg, wu, bg, bu, dz, want_dx, dw_dtype, want_bias
     dwg, dwu = (torch.empty(F, K, dtype=dw_dtype, device=x.device) for _ in range(2)) if dw_dtype is not None else (None, None)
     dbg, dbu = (torch.empty(F, dtype=torch.float32, device=x.device) for _ in range(2)) if want_bias else (None, None)
     scratch = _gated_scratch(d, x, wg, wu, 1)
-    _call('rdfc_gated_linear_backward', x, C.byref(d), _a(x), _a(wg), _a(wu), _a(bg), _a(bu), _a(dz), ld(dz), _a(scratch), _a(dx), _a(dwg), _a(dwu),
+    _call('rdfc_gated_linear_backward', x, C.byref(d), _a(x), _a(wg), _a(wu), _a(bg), _a(bu), _a(pre), _a(dz), ld(dz), _a(scratch), _a(dx), _a(dwg), _a(dwu),
           F32 if dw_dtype == torch.float32 else dt(x), _a(dbg), _a(dbu))
     return dx, dwg, dwu, dbg, dbu

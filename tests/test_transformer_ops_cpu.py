@@ -162,7 +162,7 @@ def test_c_abi_refusals():
     assert bwd(nr()) and b'null' in err()
     assert bwd(nr(rows=0)) == 0
     gl = lambda **k: hip.GatedDesc(**{**dict(M=4, K=8, F=8, ldx=8, ldwg=8, ldwu=8, dtype=1, act=16), **k})
-    fwd = lambda d: lib.rdfc_gated_linear(ctypes.byref(d), *[None] * 8)
+    fwd = lambda d: lib.rdfc_gated_linear(ctypes.byref(d), *[None] * 9)
     assert fwd(gl()) and b'null' in err()
     assert fwd(gl(act=2)) and b'activation' in err()
     assert fwd(gl(ldwu=4)) and b'ld smaller' in err()
@@ -172,7 +172,7 @@ def test_c_abi_refusals():
     assert lib.rdfc_gated_linear_scratch_bytes(ctypes.byref(gl(dtype=9)), None, None, None, 0) == 0
     assert lib.rdfc_gated_linear_scratch_bytes(ctypes.byref(gl()), 16, 32, 48, 0) == 0
     assert lib.rdfc_gated_linear_scratch_bytes(ctypes.byref(gl()), 2, 32, 48, 0) == 256
-    bwd = lambda d, lddz=8, dw=0: lib.rdfc_gated_linear_backward(ctypes.byref(d), *[None] * 6, lddz, None, None, None, None, dw, None, None, None)
+    bwd = lambda d, lddz=8, dw=0: lib.rdfc_gated_linear_backward(ctypes.byref(d), *[None] * 7, lddz, None, None, None, None, dw, None, None, None)
     assert bwd(gl()) and b'null' in err()
     assert bwd(gl(), lddz=7) and b'lddz' in err()
     assert bwd(gl(), dw=2) and b'weight gradients' in err()

@@ -544,7 +544,7 @@ int rdfc_sum_maps(int n, const void *const *srcs, const int *lds, void *dst, int
 /* y[e] = keep(e) ? x[e] / (1 - threshold / 65536) : 0 over a map of P pixels and C channels; e: the element's index in the dense
  * order.  keep(e): the 16-bit half e % 8 (low half of a word first) of the four words of Philox4x32-10 with counter (e / 8, offset) and
  * key seed is not below `threshold` (0 .. 65536).  key: device memory {seed, offset} read in place of the two arguments, or NULL.
- * The backward pass is the same call on the cotangent.  Nothing is stored.  y may be x. */
+ * The backward pass is the same call on the cotangent.  Nothing is stored. */
 int rdfc_dropout(const void *x, void *y, int64_t P, int C, int ldx, int ldy, int dtype, int threshold, uint64_t seed, uint64_t offset,
                  const uint64_t *key, void *stream);
 /* one draw of a generator state in device memory: key = {state[0], state[1]}, state[1] += 1 (both: two uint64) */
@@ -582,7 +582,7 @@ typedef struct rdfc_gated_desc {
     int64_t M;
     int32_t K, F, ldx, ldwg, ldwu, dtype, act;
 } rdfc_gated_desc;
-/* bytes of scratch (256-byte aligned) that a forward or backward call with these operands needs; the pointers' alignment counts, not what
+/* bytes of scratch (16-byte aligned) that a forward or backward call with these operands needs; the pointers' alignment counts, not what
  * they point to: rows that are not whole 16-byte vectors are copied first.  0: scratch may be NULL.
  * pre: f32 maps only, [M][2 Fp] with Fp = F rounded up to 32: g and u for the backward pass; NULL without one. */
 size_t rdfc_gated_linear_scratch_bytes(const rdfc_gated_desc *d, const void *x, const void *wg, const void *wu, int backward);

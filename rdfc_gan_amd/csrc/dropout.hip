@@ -88,10 +88,10 @@ __global__ __launch_bounds__(NT) void dropout_kernel(DropArgs d, const T *__rest
     }
 }
 
-// key = {state[0], state[1]}, state[1] += 1: one draw of a device-side generator state
+// key = {state[0], state[1]}, state[1] += 1: one draw of a device-side generator state (draws on several streams at once get keys of their own)
 __global__ void dropout_draw_kernel(unsigned long long *state, unsigned long long *key) {
     key[0] = state[0];
-    key[1] = state[1]++;
+    key[1] = atomicAdd(state + 1, 1ull);
 }
 
 }  // namespace

@@ -718,6 +718,7 @@ int check(const rdfc_gated_desc *d, const char *name) {
     RDFC_REQUIRE(rdfc_dtype_ok(d->dtype), "%s: unsupported dtype %d", name, d->dtype);
     RDFC_REQUIRE(d->M >= 0 && d->M <= (int64_t)0x7fffffff * 32 && d->K > 0 && d->F > 0 && d->F <= (1 << 20) && d->K <= (1 << 20),
                  "%s: bad sizes M=%lld K=%d F=%d", name, (long long)d->M, d->K, d->F);
+    RDFC_REQUIRE((int64_t)d->F * d->K <= (1ll << 36), "%s: weights of %d x %d are too large", name, d->F, d->K);
     RDFC_REQUIRE(d->ldx >= d->K && d->ldwg >= d->K && d->ldwu >= d->K, "%s: ld smaller than K", name);
     RDFC_REQUIRE(d->act == RDFC_ACT_RELU || d->act == RDFC_ACT_SIGMOID || d->act == RDFC_GATE_SILU || d->act == RDFC_GATE_GELU, "%s: unsupported activation %d",
                  name, d->act);
@@ -751,7 +752,7 @@ extern "C" int rdfc_gated_linear(const rdfc_gated_desc *d, const void *x, const 
     RDFC_REQUIRE(x && wg && wu && z, "rdfc_gated_linear: null pointer");
     RDFC_REQUIRE(!bg == !bu, "rdfc_gated_linear: one bias without the other");
     const Packs k = packs_of(d, x, wg, wu);
-    RDFC_REQUIRE(k.bytes() == 0 || scratch, "rdfc_gated_linear: these operands need scratch memory");
+    RDFC_REQUIRE(k.bytes() == 0 || (scratch && (reinterpret_cast<size_t>(scratch) & 15) == 0), "rdfc_gated_linear: these operands need (aligned) scratch memory");
     GLArgs p = args(d, x, wg, wu, bg, bu);
     if (pack(d, k, p, scratch, (hipStream_t)stream, "rdfc_gated_linear (pack)")) return 2;
     RDFC_REQUIRE(!pre || (d->dtype == RDFC_F32 && (reinterpret_cast<size_t>(pre) & 15) == 0), "rdfc_gated_linear: pre is kept for f32 maps, 16-byte aligned");
@@ -777,6 +778,7 @@ extern "C" int rdfc_gated_linear_backward(const rdfc_gated_desc *d, const void *
     RDFC_REQUIRE(!bg == !bu, "rdfc_gated_linear_backward: one bias without the other");
     RDFC_REQUIRE(dw_dtype == RDFC_F32 || dw_dtype == d->dtype, "rdfc_gated_linear_backward: weight gradients are f32 or of the map's type");
     RDFC_REQUIRE(wg && wu && (d->M == 0 || (x && dz && scratch)), "rdfc_gated_linear_backward: null pointer");
+    RDFC_REQUIRE(((reinterpret_cast<size_t>(scratch) | reinterpret_cast<size_t>(pre)) & 15) == 0, "rdfc_gated_linear_backward: scratch or pre is not 16-byte aligned");
     const Plan q = plan_of(d);
     const Packs k = packs_of(d, x, wg, wu);
     const hipStream_t st = (hipStream_t)stream;

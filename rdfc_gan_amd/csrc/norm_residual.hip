@@ -34,7 +34,7 @@ struct NRArgs {
     int64_t rows;                    // per sample
     int C, ldx, ldh, ldy, ldn, lddy, lddn;
     const float *gate, *scale, *post_w, *post_b, *pre_w, *pre_b;
-    int layer, post, pre;
+    int layer, post, pre, par_al;    // par_al: every parameter vector is 16-byte aligned
     float eps;
     DropArgs drop;
     f32x4 *stats;                    // per row: mean and reciprocal deviation of h, of y
@@ -135,8 +135,8 @@ template <typename T, bool ALIGNED> __device__ __forceinline__ void store8(const
     }
 }
 // a parameter vector (f32); a null pointer stands for `none`.  0 beyond C: what the lanes behind the last channel hold must not enter a sum
-template <bool ALIGNED> __device__ __forceinline__ void load_par(float (&v)[8], const float *p, int c, int C, float none) {
-    if (ALIGNED && p != nullptr && c < C) {
+template <bool ALIGNED> __device__ __forceinline__ void load_par(float (&v)[8], const float *p, int c, int C, float none, int par_al) {
+    if (ALIGNED && par_al && p != nullptr && c < C) {
         const f32x4 a = *reinterpret_cast<const f32x4 *>(p + c), b = *reinterpret_cast<const f32x4 *>(p + c + 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
@@ -151,10 +151,10 @@ template <int LPR, int VPL, bool ALIGNED> __device__ __forceinline__ void load_f
     for (int v = 0; v < VPL; ++v) {
         const int c = (v * LPR + li) * 8;
         float s[8], g[8];
-        load_par<ALIGNED>(s, p.scale, c, p.C, 1.f);
-        load_par<ALIGNED>(g, p.gate ? p.gate + (size_t)blockIdx.y * p.C : nullptr, c, p.C, 1.f);
-        load_par<ALIGNED>(fw[v], p.post_w, c, p.C, 1.f);
-        load_par<ALIGNED>(fb[v], p.post_b, c, p.C, 0.f);
+        load_par<ALIGNED>(s, p.scale, c, p.C, 1.f, p.par_al);
+        load_par<ALIGNED>(g, p.gate ? p.gate + (size_t)blockIdx.y * p.C : nullptr, c, p.C, 1.f, p.par_al);
+        load_par<ALIGNED>(fw[v], p.post_w, c, p.C, 1.f, p.par_al);
+        load_par<ALIGNED>(fb[v], p.post_b, c, p.C, 0.f, p.par_al);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             fw[v][i] *= s[i] * g[i];
@@ -175,8 +175,8 @@ __global__ __launch_bounds__(threads_of(LPR), VPL == 1 ? (sizeof(T) == 2 ? 5 : 4
     load_factors<LPR, VPL, ALIGNED>(p, li, fw, fb);
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
-        load_par<ALIGNED>(qw[v], p.pre_w, (v * LPR + li) * 8, C, 1.f);
-        load_par<ALIGNED>(qb[v], p.pre_b, (v * LPR + li) * 8, C, 0.f);
+        load_par<ALIGNED>(qw[v], p.pre_w, (v * LPR + li) * 8, C, 1.f, p.par_al);
+        load_par<ALIGNED>(qb[v], p.pre_b, (v * LPR + li) * 8, C, 0.f, p.par_al);
     }
     const int64_t r0 = (int64_t)blockIdx.x * p.chunk, r1 = min(r0 + p.chunk, p.rows), base = (int64_t)blockIdx.y * p.rows;
     // mean and reciprocal deviation of the row in a[][]; a[][] becomes the normalised row
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(threads_of(LPR), VPL == 1 ? (sizeof(T) == 2 ? 3 : 2
     load_factors<LPR, VPL, ALIGNED>(p, li, fw, fb);
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
-        load_par<ALIGNED>(qw[v], p.pre_w, (v * LPR + li) * 8, C, 1.f);
+        load_par<ALIGNED>(qw[v], p.pre_w, (v * LPR + li) * 8, C, 1.f, p.par_al);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -578,6 +578,7 @@ static NRArgs nr_args(const rdfc_norm_residual_desc *d, const void *x, const voi
     p.post = d->post && h != nullptr;
     p.pre = d->pre;
     p.eps = d->eps;
+    p.par_al = par_aligned({gate, scale, post_w, post_b, pre_w, pre_b});
     drop_args(p.drop, d->threshold, d->seed, d->offset, key);
     return p;
 }
@@ -587,6 +588,7 @@ extern "C" int rdfc_norm_residual(const rdfc_norm_residual_desc *d, const void *
                                   void *n, float *stats, void *stream) {
     if (nr_check(d, "rdfc_norm_residual")) return 1;
     if (d->samples == 0 || d->rows == 0) return 0;
+    RDFC_REQUIRE((reinterpret_cast<size_t>(stats) & 15) == 0, "rdfc_norm_residual: stats is not 16-byte aligned");
     RDFC_REQUIRE(x && (h ? y != nullptr : (d->pre && !gate && !scale)) && (!d->pre || n), "rdfc_norm_residual: null map");
     NRArgs p = nr_args(d, x, h, gate, scale, post_w, post_b, pre_w, pre_b, key);
     p.y = y;
@@ -598,8 +600,7 @@ extern "C" int rdfc_norm_residual(const rdfc_norm_residual_desc *d, const void *
     p.rows = gate ? d->rows : d->rows * d->samples;
     p.chunk = chunk_of(p.rows, samples, d->C, FWD_GROUPS);
     const dim3 grid((unsigned)((p.rows + p.chunk - 1) / p.chunk), samples);
-    const bool al = row_aligned(x, d->ldx, d->dtype) && row_aligned(h, d->ldh, d->dtype) && row_aligned(y, d->C, d->dtype) && row_aligned(n, d->C, d->dtype) && d->C % 8 == 0 &&
-                    par_aligned({gate, scale, post_w, post_b, pre_w, pre_b});
+    const bool al = row_aligned(x, d->ldx, d->dtype) && row_aligned(h, d->ldh, d->dtype) && row_aligned(y, d->C, d->dtype) && row_aligned(n, d->C, d->dtype) && d->C % 8 == 0;
     with_layout(d->C, [&](auto lpr, auto vpl) {
         constexpr int L = decltype(lpr)::value, V = decltype(vpl)::value;
         RDFC_DISPATCH(d->dtype, if (al) norm_residual_kernel<T, L, V, true><<<grid, threads_of(L), 0, (hipStream_t)stream>>>(p);
@@ -627,6 +628,7 @@ extern "C" int rdfc_norm_residual_backward(const rdfc_norm_residual_desc *d, con
     const bool empty = d->samples == 0 || d->rows == 0;
     if (empty && !cols) return 0;
     if (!empty) RDFC_REQUIRE(x && dx && (!h || dh) && stats && (!dn || d->pre) && (!cols || scratch), "rdfc_norm_residual_backward: null pointer");
+    RDFC_REQUIRE(((reinterpret_cast<size_t>(stats) & 15) | (reinterpret_cast<size_t>(scratch) & 7)) == 0, "rdfc_norm_residual_backward: stats or scratch is not aligned");
     RDFC_REQUIRE(!d_gate || gate, "rdfc_norm_residual_backward: gradient of a gate that is not there");
     NRArgs p = nr_args(d, x, h, gate, scale, post_w, post_b, pre_w, nullptr, key);
     p.dy = dy;
@@ -645,8 +647,7 @@ extern "C" int rdfc_norm_residual_backward(const rdfc_norm_residual_desc *d, con
         p.chunk = k.chunk;
         const dim3 grid((unsigned)k.nchunk, samples);
         const bool al = row_aligned(x, d->ldx, d->dtype) && row_aligned(h, d->ldh, d->dtype) && row_aligned(dy, lddy, d->dtype) &&
-                        row_aligned(dn, lddn, d->dtype) && row_aligned(dx, d->C, d->dtype) && row_aligned(dh, d->C, d->dtype) && d->C % 8 == 0 &&
-                        par_aligned({gate, scale, post_w, post_b, pre_w});
+                        row_aligned(dn, lddn, d->dtype) && row_aligned(dx, d->C, d->dtype) && row_aligned(dh, d->C, d->dtype) && d->C % 8 == 0;
         with_layout(d->C, [&](auto lpr, auto vpl) {
             constexpr int L = decltype(lpr)::value, V = decltype(vpl)::value;
             RDFC_DISPATCH(d->dtype, if (al) norm_residual_bwd_kernel<T, L, V, true><<<grid, threads_of(L), 0, (hipStream_t)stream>>>(p);

@@ -728,6 +728,11 @@ class RDFCGAN:
         if enabled:
             for o in self.optimizers.values():
                 o.make_capturable()
+            # (elementwise dropout inside a captured step draws from a state in device memory: every replay its own masks)
+            for net in (self.G_A2B, self.G_B2A):
+                for m in net.modules():
+                    if isinstance(m, layers.Dropout) and m.rng is None:
+                        m.rng = Fh.DropoutState(device=self.device)
 
     def _mask_to_device(self, mask):
         """host mask -> device through a pinned staging buffer: a pageable-memory copy makes the host wait for every kernel

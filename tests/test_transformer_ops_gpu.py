@@ -153,6 +153,34 @@ def test_dropout_without_a_state_is_refused_in_a_graph():
     assert torch.equal(y, x + 1)
 
 
+def test_dropout_state_on_two_streams_at_once():
+    """draws that overlap get keys of their own"""
+    state = Fh().DropoutState(3, torch.device(DEV, torch.cuda.current_device()))
+    torch.cuda.synchronize()
+    keys, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    for i in range(40):
+        with torch.cuda.stream(streams[i % 2]):
+            keys.append(state.draw())
+    torch.cuda.synchronize()
+    assert sorted(int(k[1]) for k in keys) == list(range(40)) and int(state.state[1]) == 40
+
+
+def test_dropout_beyond_32_bit_indexes():
+    """a map of more than 2^32 elements: the last elements against the oracle's window of the mask"""
+    shape = (1, 8193, 8192, 64)
+    x = torch.ones(shape, dtype=torch.bfloat16, device=DEV)
+    n = x.numel()
+    assert n > 1 << 32
+    y = Fh().dropout(x, 0.5, rng=(7, 1 << 60)).view(-1)
+    for first in (0, (1 << 32) - 5000, (1 << 32) - 8, n - 100_003):
+        m = min(10_000, n - first)
+        assert torch.equal(y[first:first + m].cpu() != 0, O.keep_mask(m, 1 << 15, 7, 1 << 60, first=first)), first
+    del y
+    y = Fh().dropout(x[..., :63], 0.25, rng=(7, 8))                   # element by element, 64-bit rows
+    first = y.numel() - 9_999
+    assert torch.equal(y.view(-1)[first:].cpu() != 0, O.keep_mask(9_999, 1 << 14, 7, 8, first=first))
+
+
 # ---- norm_residual --------------------------------------------------------------------------------------------------------
 def residual_case(shape, dtype, how, layer, post, pre, gated, scaled, p, seed=0, dy=True, dn=True):
     """runs norm_residual with its gradients and holds every output against the oracle"""
@@ -263,6 +291,35 @@ def test_row_norm():
             check(t, *want[k], k)
 
 
+def test_norm_residual_misaligned_parameters():
+    """parameters inside a flat buffer (as an optimizer lays them out), at offsets that are not whole vectors"""
+    C = 64
+    x, h = rnd(2, 3, 5, C, seed=1).to(DEV), rnd(2, 3, 5, C, seed=2).to(DEV)
+    flat = rnd(4 * C + 1, seed=3).to(DEV)
+    v = [flat[1 + i * C:1 + (i + 1) * C] for i in range(4)]
+    a = Fh().norm_residual(x, h, scale=v[0], post=(v[1], v[2]), pre=(v[3], None))
+    b = Fh().norm_residual(x, h, scale=v[0].clone(), post=(v[1].clone(), v[2].clone()), pre=(v[3].clone(), None))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_norm_residual_beyond_32_bit_indexes():
+    """maps of more than 2^32 elements: the last rows are those of a small call on them, and their dropout the oracle's window"""
+    shape, tail = (1, 8193, 8192, 64), 5000
+    x = torch.zeros(shape, dtype=torch.bfloat16, device=DEV)
+    h = torch.zeros(shape, dtype=torch.bfloat16, device=DEV)
+    for t, seed in ((x, 1), (h, 2)):
+        t.view(-1, 64)[-tail:] = rnd(tail, 64, seed=seed, dtype=torch.bfloat16).to(DEV)
+    small = [t.view(-1, 64)[-tail:].reshape(1, 1, tail, 64) for t in (x, h)]
+    w = rnd(64, seed=3, mean=1.0).to(DEV)
+    y, n = Fh().norm_residual(x, h, post=(w, None), pre=(w, None))
+    ys, ns = Fh().norm_residual(*small, post=(w, None), pre=(w, None))
+    assert torch.equal(y.view(-1, 64)[-tail:], ys.view(-1, 64)) and torch.equal(n.view(-1, 64)[-tail:], ns.view(-1, 64))
+    del y, n
+    y, _ = Fh().norm_residual(torch.zeros_like(x), torch.ones_like(h), p=0.5, rng=(5, 6))
+    first = x.numel() - tail * 64
+    assert torch.equal(y.view(-1)[first:].cpu() != 0, O.keep_mask(tail * 64, 1 << 15, 5, 6, first=first))
+
+
 def test_norm_residual_empty_and_unused():
     x = torch.zeros(2, 0, 4, 8, device=DEV, requires_grad=True)
     w = torch.ones(8, device=DEV, requires_grad=True)
@@ -336,6 +393,26 @@ def test_gated_linear_weights_of_a_1x1_convolution_and_of_one_matrix():
     wide = torch.zeros(40, 31, device=DEV)
     wide[:, 3:27] = w[0]
     assert torch.equal(z, Fh().gated_linear(x, wide[:, 3:27], w[1]))
+
+
+def test_gated_linear_beyond_32_bit_indexes():
+    """a map of more than 2^32 elements: the last rows are those of a small call on them"""
+    M, K, F, tail = (1 << 24) + 77, 264, 16, 500
+    x = torch.zeros(1, 1, M, K, dtype=torch.bfloat16, device=DEV)
+    x[0, 0, -tail:] = rnd(tail, K, seed=1, dtype=torch.bfloat16).to(DEV)
+    w = [rnd(F, K, seed=2 + i, std=0.1, dtype=torch.bfloat16).to(DEV) for i in range(2)]
+    assert x.numel() > 1 << 32
+    z = Fh().gated_linear(x, *w)
+    assert torch.equal(z[0, 0, -tail:], Fh().gated_linear(x[:, :, -tail:].contiguous(), *w)[0, 0])
+    assert not bool(z[0, 0, :1000].any())
+
+
+def test_gated_linear_takes_expanded_cotangents_and_runs_backward_twice():
+    x, w = rnd(1, 5, 6, 24, seed=1).to(DEV).requires_grad_(True), rnd(2, 40, 24, seed=2).to(DEV).requires_grad_(True)
+    z = Fh().gated_linear(x, w[0], w[1])
+    a = torch.autograd.grad(z.sum(), [x, w], retain_graph=True)
+    b = torch.autograd.grad(z, [x, w], torch.ones_like(z))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
 def test_gated_linear_extreme_gates():
@@ -481,6 +558,61 @@ def test_trunk_trains_in_16_bits_and_replays_from_a_graph():
             else:
                 assert torch.equal(a, b), (rep, name)
         torch.cuda.synchronize()
+
+
+def test_trunk_under_the_flat_optimizer():
+    """a step of FlatAdam on a bf16 trunk of odd hidden width, f32 masters in its flat buffer: gradients land there, weights move, and the
+    next forward uses them"""
+    from rdfc_gan_amd.layers import GatedFeedForwardTrunk
+    from rdfc_gan_amd.optim import FlatAdam
+    torch.manual_seed(7)
+    trunk = GatedFeedForwardTrunk(2, 36, 45, p=0.1, bias=True, scale=1.0).to(DEV)
+    x = rnd(2, 6, 5, 36, seed=1, dtype=torch.bfloat16).to(DEV)
+    opt = FlatAdam(trunk.parameters(), lr=1e-2)
+    before = [p.detach().clone() for p in trunk.parameters()]
+    first = trunk.eval()(x)
+    opt.zero_grad()
+    trunk.train()(x).float().square().mean().backward()
+    opt.step()
+    for (k, p), b in zip(trunk.named_parameters(), before):
+        unused = k == 'blocks.0.pre.bias'
+        assert bool(torch.isfinite(p).all()) and (unused or not torch.equal(p.detach(), b)), k
+    assert not torch.equal(first, trunk.eval()(x))
+
+
+def test_graph_mode_with_dropout():
+    """RDFCGAN.enable_graph() with a dropout generator: the replayed steps run and draw a new mask each"""
+    from cases import STEP_HP, step_batch
+    from rdfc_gan_amd import functional
+    from rdfc_gan_amd.rdfc_gan import RDFCGAN
+    old = functional.compute_dtype()
+    functional.set_compute_dtype(torch.float16)
+    try:
+        norm = dict(norm_cfg=dict(type='BN2d'), activation='LeakyReLU')
+        cfg = dict(local_rank=0, lr=2e-3, beta1=0.5, beta2=0.999, gan_loss_type='lsgan',
+                   model=dict(G_A2B=dict(type='RDFGenerator', pretrained_on_imagenet=False),
+                              G_B2A=dict(type='ResnetGenerator', input_channels=1, output_channels=3, ngf=64, norm_layer='IN2d', use_dropout=True),
+                              D_A=dict(type='PatchGANDiscriminator', in_channels=1, **norm), D_B=dict(type='PatchGANDiscriminator', in_channels=3, **norm)))
+        m = RDFCGAN(torch.device(DEV), False, cfg, is_train=True)
+        m.train()
+        data, nA, _ = step_batch(0, 2, STEP_HP['H'], STEP_HP['W'])
+        data['gt_normal'] = nA
+        counts = []
+        for it in range(5):                              # (two eager steps first: the convolutions' own buffers cannot be allocated in a capture)
+            if it == 2:
+                m.enable_graph(True)
+                state = next(d for d in m.G_B2A.modules() if isinstance(d, torch.nn.Dropout)).rng.state
+            m.set_input(data)
+            losses = m.optimize_parameters()
+            assert all(v == v and abs(v) < 1e6 for v in losses.values()), losses
+            torch.cuda.synchronize()
+            if it >= 2:
+                counts.append(int(state[1]))
+        assert m._graph_mode and m._graphs is not None, 'capture fell back to eager launches'
+        assert counts[2] > counts[1] > counts[0] > 0, counts
+        m.enable_graph(False)
+    finally:
+        functional.set_compute_dtype(old)
 
 
 def test_generator_with_dropout():

@@ -98,10 +98,15 @@ template <typename T> __global__ __launch_bounds__(NT) void gated_pack_kernel(co
 
 // ---- the tiled kernel --------------------------------------------------------------------------------------------------------------
 // Four waves, each WTP x WTQ of a (2 WTP) x (2 WTQ) tile; operands go global -> LDS by LDS-DMA (buffer_load ... lds) into a ring of three
-// K-steps of 64 bytes a row, filled two steps ahead; one raw barrier and one counted wait per step.  At 128 x 64 a wave and step issues
-// 32 MFMAs (512 cycles of its SIMD) on 12 KB of LDS reads, the workgroup 24 KB of DMA: 576 cycles of LDS for 512 of MFMA per pair of
-// steps on a CU, and two workgroups (72 KB of LDS each) share a CU, so that one's prologue and epilogue -- as long as the K loop at
-// K = 256: 64 activations a lane -- run under the other's MFMAs.
+// K-steps of 64 bytes a row, filled two steps ahead; one raw barrier and one counted wait per step.  A 64 x 64 wave tile needs 48 KB of LDS and
+// 107 registers: three workgroups share a CU, and one's prologue and epilogue run under the others' MFMAs.  That matters more here than a
+// cheaper K loop: at K = 256 half of the forward pass's time is not the K loop (one K-step instead of eight: 33 of 64 us).
+//
+// Measured (16-bit): forward 34656 x 256 -> 1024 60 us, 605 TFLOP/s (a library product of the same size without activation: 73 us);
+// 8816 x 512 -> 2048 52 us (library 79); 34656 x 1024 -> 1024 160 us, 908 TFLOP/s, where the matrix pipes are busy for half of the cycles.  Backward
+// of the first: D 84, dx 49, dW 46 and its join 13, bias join 5 us.
+// Tried and not kept: fragments read a step ahead in a second register set (no change), steps of 128 bytes in two pairs of slots (two
+// workgroups a CU: 60 -> 70 us at K = 256), eight waves on 256 x 128 with a ring of three 128-byte steps (75 us at K = 256, 174 at K = 1024).
 //
 // An operand whose contraction index is contiguous in memory (ROW) has an LDS image [row][64 bytes], the 16-byte chunk c of row r at c ^ (r >> 1 & 3):
 // eight lanes of a fragment read (rows r .. r + 7, one chunk) then cover all 128 bytes of the banks.  One whose contraction index is the

@@ -10,6 +10,10 @@
 // same bytes as reading a saved y) in f32, so neither y nor the dropout mask nor the normalised maps are kept -- four f32 statistics
 // per pixel are.
 //
+// Measured: 8x57x76x1024 f16 (layer norm before the next block) 54 us forward, 284 MB at 5.3 TB/s, and 110 backward, 426 MB at 3.9 TB/s: three
+// waves a SIMD, 168 registers (the sums alone are 32), leave fewer loads under way than the forward pass's five waves.  8x57x76x256 bf16, both
+// norms, gate and dropout: 18 and 25 us, column sums 8.
+//
 // Column sums (gradients of the four norm parameters, of scale and of gate) reduce to four sums per sample and channel:
 //     A = sum D t hhat,  B = sum D t   (t: cotangent of y, D: dropout factor, hhat: normalised h, or h itself without N_post)
 //     P = sum dn yhat,   Q = sum dn

@@ -1119,6 +1119,9 @@ def norm_residual(x, h, gate, scale, post, pre, layer, eps, threshold, seed, off
     return d, y, n, stats
 
 
+_nr_scratch = {}         # sizes -> floats of scratch
+
+
 def norm_residual_backward(d, x, h, gate, scale, post, pre, key, stats, dy, dn, want):
     """want: which of (gate, scale, post_w, post_b, pre_w, pre_b) need a gradient -> (dx, dh, those six)"""
     N, H, W, Cc = x.shape
@@ -1132,7 +1135,11 @@ def norm_residual_backward(d, x, h, gate, scale, post, pre, key, stats, dy, dn, 
         sizes = [(N if i == 0 else 1) * Cc for i, w in enumerate(want) if w]
         flat = iter(torch.empty(sum(sizes), dtype=torch.float32, device=x.device).split(sizes))
         cols = [(next(flat).view(N, Cc) if i == 0 else next(flat)) if w else None for i, w in enumerate(want)]
-        scratch = torch.empty(lib().rdfc_norm_residual_scratch_floats(C.byref(d), int(gate is not None)), dtype=torch.float32, device=x.device)
+        key_ = (d.rows, d.samples, Cc, gate is not None)
+        n = _nr_scratch.get(key_)
+        if n is None:
+            n = _nr_scratch[key_] = lib().rdfc_norm_residual_scratch_floats(C.byref(d), int(gate is not None))
+        scratch = torch.empty(n, dtype=torch.float32, device=x.device)
     _call('rdfc_norm_residual_backward', x, C.byref(d), _a(x), _a(h), _a(gate), _a(scale), _a(pw), _a(pb), _a(qw), _a(key), _a(stats), _a(dy),
           ld(dy) if dy is not None else Cc, _a(dn), ld(dn) if dn is not None else Cc, _a(dx), _a(dh), _a(scratch), *map(_a, cols))
     return (dx, dh, *cols)

@@ -402,8 +402,9 @@ __global__ __launch_bounds__(threads_of(LPR), VPL == 1 ? (sizeof(T) == 2 ? 3 : 2
         for (int v = 0; v < VPL; ++v)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float d = keep[v] >> i & 1 ? t[v][i] * p.drop.inv : 0.f;
-                sum[0][v][i] = fmaf(d, hat[v][i], sum[0][v][i]);
+                const bool kept = keep[v] >> i & 1;
+                const float d = kept ? t[v][i] * p.drop.inv : 0.f;
+                sum[0][v][i] = kept ? fmaf(d, hat[v][i], sum[0][v][i]) : sum[0][v][i];      // (a dropped element may hold anything)
                 sum[1][v][i] += d;
                 t[v][i] = d * fw[v][i];
             }

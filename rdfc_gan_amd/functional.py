@@ -16,6 +16,7 @@ Blocks
 """
 import math
 import os
+import threading
 import weakref
 
 import torch
@@ -1037,6 +1038,9 @@ class DropoutState:
         return hip.dropout_draw(self.state)
 
 
+_generator_lock = threading.Lock()
+
+
 def _signed64(v):
     v &= 0xffffffffffffffff
     return v - (1 << 64) if v >> 63 else v
@@ -1065,8 +1069,9 @@ def _drop_rng(p, training, rng, x):
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError('dropout inside a HIP graph: pass rng=DropoutState(...) (torch\'s generator would give every replay the same mask)')
     gen = torch.cuda.default_generators[device.index]
-    at = gen.get_offset()
-    gen.set_offset(at + 4)
+    with _generator_lock:
+        at = gen.get_offset()
+        gen.set_offset(at + 4)
     return threshold, gen.initial_seed() & 0xffffffffffffffff, 1 << 63 | at, None        # (bit 63: apart from the counters of torch's own kernels)
 
 

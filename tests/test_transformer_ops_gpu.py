@@ -104,6 +104,27 @@ def test_dropout_from_torchs_generator():
     assert abs(float((a == 0).float().mean()) - 0.4) < 5 * (0.24 / a.numel()) ** 0.5
 
 
+def test_dropout_from_several_threads():
+    """every call takes an offset of its own"""
+    import threading
+    x = torch.ones(1, 4, 4, 64, device=DEV)
+    out, gate = [], threading.Barrier(4)
+
+    def work():
+        gate.wait()
+        for _ in range(20):
+            out.append(Fh().dropout(x, 0.5))
+    torch.manual_seed(11)
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    masks = {bytes((o != 0).cpu().numpy().tobytes()) for o in out}
+    assert len(out) == 80 and len(masks) == 80
+
+
 def test_dropout_empty_map():
     x = torch.zeros(0, 3, 4, 8, device=DEV, requires_grad=True)
     y = Fh().dropout(x, 0.5, rng=(1, 2))
@@ -289,6 +310,35 @@ def test_row_norm():
         check(n, *want['n'], 'n')
         for t, k in zip(torch.autograd.grad(n, leaves, g.to(DEV)), ('x', 'pre_w', 'pre_b')):
             check(t, *want[k], k)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+def test_norm_residual_hides_what_it_drops(dtype):
+    """NaN and infinities in dropped places of h reach neither the maps nor a gradient"""
+    shape, rng = (2, 3, 5, 40), (5, 6)
+    keep = O.keep_mask(2 * 3 * 5 * 40, O.threshold_of(0.4), *rng).view(shape)
+    x, h, gy = (rnd(*shape, seed=i, dtype=dtype) for i in range(3))
+    scale, gate = rnd(40, seed=4), rnd(2, 40, seed=5)
+    bad = torch.where(keep, h, torch.full_like(h, float('nan')))
+    bad[0, 0] = torch.where(keep[0, 0], h[0, 0], torch.full_like(h[0, 0], float('inf')))
+    outs = []
+    for t in (h, bad):
+        v = [a.to(DEV).detach().requires_grad_(True) for a in (x, t, gate, scale)]
+        y, _ = Fh().norm_residual(v[0], v[1], gate=v[2], scale=v[3], p=0.4, rng=rng)
+        outs.append([y, *torch.autograd.grad(y, v, gy.to(DEV))])
+    for a, b in zip(*outs):
+        assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
+
+
+def test_norm_residual_takes_activations_as_gate_and_scale():
+    """a 16-bit gate [N, 1, 1, C] that another layer produced gets its gradient in its own type"""
+    x, h = rnd(2, 3, 4, 24, seed=1, dtype=torch.bfloat16).to(DEV), rnd(2, 3, 4, 24, seed=2, dtype=torch.bfloat16).to(DEV)
+    gate = rnd(2, 1, 1, 24, seed=3, dtype=torch.bfloat16).to(DEV).requires_grad_(True)
+    y, _ = Fh().norm_residual(x, h, gate=gate)
+    f = gate.detach().float().flatten(1).requires_grad_(True)
+    z, _ = Fh().norm_residual(x, h, gate=f)
+    a, b = torch.autograd.grad(y, gate, torch.ones_like(y))[0], torch.autograd.grad(z, f, torch.ones_like(z))[0]
+    assert torch.equal(y, z) and a.dtype == torch.bfloat16 and a.shape == gate.shape and torch.equal(a.flatten(1), b.to(torch.bfloat16))
 
 
 def test_norm_residual_misaligned_parameters():

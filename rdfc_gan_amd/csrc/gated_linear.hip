@@ -562,16 +562,29 @@ __global__ __launch_bounds__(NT) void gated_act_kernel(GLArgs p) {
         p.partial[(size_t)blockIdx.x * 2 * p.Fp + k * p.Fp + c] = (red[0][k][threadIdx.x] + red[1][k][threadIdx.x]) + (red[2][k][threadIdx.x] + red[3][k][threadIdx.x]);
 }
 
-// o0 (o1: the second half of a part) [n] = sum over the parts of partial[part][step], in the order of the parts, in f64
-template <typename TO> __global__ __launch_bounds__(NT) void gated_join_kernel(const float *__restrict__ partial, int parts, size_t n, size_t step, TO *o0, TO *o1) {
-    const size_t i = (size_t)blockIdx.x * NT + threadIdx.x;
+// o0 (o1: the second half of a part) [n] = sum over the parts of partial[part][step], in the order of the parts, in f64.  V elements a thread
+template <typename TO, int V> __global__ __launch_bounds__(NT) void gated_join_kernel(const float *__restrict__ partial, int parts, size_t n, size_t step, TO *o0, TO *o1) {
+    const size_t i = ((size_t)blockIdx.x * NT + threadIdx.x) * V;
     TO *o = blockIdx.y ? o1 : o0;
     if (i >= n || o == nullptr) return;
     const float *src = partial + i + (blockIdx.y ? step / 2 : 0);
-    double s = 0.;
+    double s[V] = {};
 #pragma unroll 8
-    for (int k = 0; k < parts; ++k) s += (double)src[k * step];
-    Elem<TO>::st(o + i, (float)s);
+    for (int k = 0; k < parts; ++k) {
+        if constexpr (V == 4) {
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(src + k * step);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[r] += (double)v[r];
+        } else {
+            s[0] += (double)src[k * step];
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < V; ++r) Elem<TO>::st(o + i + r, (float)s[r]);
+}
+template <typename TO> void join(const float *partial, int parts, size_t n, size_t step, TO *o0, TO *o1, int halves, hipStream_t st) {
+    if (n % 4 == 0 && step % 8 == 0) gated_join_kernel<TO, 4><<<dim3((unsigned)((n / 4 + NT - 1) / NT), halves), NT, 0, st>>>(partial, parts, n, step, o0, o1);
+    else gated_join_kernel<TO, 1><<<dim3((unsigned)((n + NT - 1) / NT), halves), NT, 0, st>>>(partial, parts, n, step, o0, o1);
 }
 
 // out[kind][f] = sum over the row blocks of partial[block][kind * Fp + f]: 32 columns x 16 row lanes per workgroup
@@ -813,7 +826,7 @@ extern "C" int rdfc_gated_linear_backward(const rdfc_gated_desc *d, const void *
             if (launch_dma<DX>(p, d->dtype, q.dx, cdiv(d->K, 2 * q.dx.wtp) * q.dx_splits, cdiv(d->M, 2 * q.dx.wtq), st, "rdfc_gated_linear_backward (input)")) return 2;
             if (q.dx_splits > 1) {
                 const size_t n = (size_t)d->M * d->K;
-                RDFC_DISPATCH(d->dtype, (gated_join_kernel<T><<<dim3((unsigned)((n + NT - 1) / NT), 1), NT, 0, st>>>(w, q.dx_splits, n, n, (T *)dx, nullptr)));
+                RDFC_DISPATCH(d->dtype, (join<T>(w, q.dx_splits, n, n, (T *)dx, nullptr, 1, st)));
                 RDFC_LAUNCH_CHECK("rdfc_gated_linear_backward (input join)");
             }
         }
@@ -830,8 +843,7 @@ extern "C" int rdfc_gated_linear_backward(const rdfc_gated_desc *d, const void *
         RDFC_LAUNCH_CHECK("rdfc_gated_linear_backward (bias join)");
     }
     if (dwg || dwu) {
-        const dim3 grid((unsigned)(((size_t)d->F * d->K + NT - 1) / NT), 2);
-        RDFC_DISPATCH(dw_dtype, (gated_join_kernel<T><<<grid, NT, 0, st>>>(w, d->M > 0 ? q.splits : 0, (size_t)d->F * d->K, (size_t)2 * q.Fp * d->K, (T *)dwg, (T *)dwu)));
+        RDFC_DISPATCH(dw_dtype, (join<T>(w, d->M > 0 ? q.splits : 0, (size_t)d->F * d->K, (size_t)2 * q.Fp * d->K, (T *)dwg, (T *)dwu, 2, st)));
         RDFC_LAUNCH_CHECK("rdfc_gated_linear_backward (join)");
     }
     return 0;

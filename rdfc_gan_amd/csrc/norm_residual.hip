@@ -10,9 +10,9 @@
 // same bytes as reading a saved y) in f32, so neither y nor the dropout mask nor the normalised maps are kept -- four f32 statistics
 // per pixel are.
 //
-// Measured: 8x57x76x1024 f16 (layer norm before the next block) 54 us forward, 284 MB at 5.3 TB/s, and 110 backward, 426 MB at 3.9 TB/s: three
-// waves a SIMD, 168 registers (the sums alone are 32), leave fewer loads under way than the forward pass's five waves.  8x57x76x256 bf16, both
-// norms, gate and dropout: 18 and 25 us, column sums 8.
+// Measured: 8x57x76x1024 f16 (layer norm before the next block) 51 us forward, 284 MB at 5.6 TB/s, and 101 backward, 426 MB at 4.2 TB/s (two waves a
+// SIMD: 180 registers, the sums alone are 32; a second row fetched ahead changes nothing), column sums 10.  8x57x76x256 bf16, both norms, gate
+// and dropout: 16 us forward, 31 backward with the column sums.
 //
 // Column sums (gradients of the four norm parameters, of scale and of gate) reduce to four sums per sample and channel:
 //     A = sum D t hhat,  B = sum D t   (t: cotangent of y, D: dropout factor, hhat: normalised h, or h itself without N_post)
@@ -26,8 +26,8 @@
 
 namespace {
 
-// threads of a workgroup: four waves, or the two that share a row of up to 1024 channels (one vector a lane keeps the backward kernel at three
-// waves per SIMD; two vectors a lane of one wave need 300 registers)
+// threads of a workgroup: four waves, or the two that share a row of up to 1024 channels (two vectors a lane of one wave would need 300 registers in
+// the backward kernel)
 constexpr int threads_of(int lpr) { return lpr == 128 ? 128 : 256; }
 
 struct NRArgs {
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(threads_of(LPR), VPL == 1 ? (sizeof(T) == 2 ? 5 : 4
 }
 
 template <typename T, int LPR, int VPL, bool ALIGNED>
-__global__ __launch_bounds__(threads_of(LPR), VPL == 1 ? (sizeof(T) == 2 ? 3 : 2) : 1) void norm_residual_bwd_kernel(NRArgs p) {
+__global__ __launch_bounds__(threads_of(LPR), VPL == 1 ? 2 : 1) void norm_residual_bwd_kernel(NRArgs p) {
     constexpr int NT = threads_of(LPR), RPB = NT / LPR;
     __shared__ float buf[2][8];
     __shared__ float red[LPR <= 64 ? 4 : 1][LPR <= 64 ? LPR * VPL * 8 : 1];
@@ -531,7 +531,9 @@ int64_t chunk_of(int64_t rows, int samples, int C, int groups) {
     while ((rows + per - 1) / per >= (1 << 20)) per *= 2;
     return per;
 }
-constexpr int FWD_GROUPS = 1280, BWD_GROUPS = 768;
+// (both: what the chip holds at once -- five and two waves a SIMD -- in one round.  The backward kernel at three waves spills, and a second round that is
+// not full costs more than the waves give: x1024 f16 at 768 / 512 workgroups of three / two waves 127 / 111 us)
+constexpr int FWD_GROUPS = 1280, BWD_GROUPS = 512;
 struct NRChunks {
     int64_t chunk;
     int nchunk, slices;

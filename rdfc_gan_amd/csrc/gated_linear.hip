@@ -104,7 +104,7 @@ template <typename T> __global__ __launch_bounds__(NT) void gated_pack_kernel(co
 //
 // Measured (16-bit): forward 34656 x 256 -> 1024 60 us, 605 TFLOP/s (a library product of the same size without activation: 73 us);
 // 8816 x 512 -> 2048 52 us (library 79); 34656 x 1024 -> 1024 160 us, 908 TFLOP/s, where the matrix pipes are busy for half of the cycles.  Backward
-// of the first: D 84, dx 49, dW 46 and its join 13, bias join 5 us.
+// of the first: D 79 (84 with dz read eight bytes a lane in the epilogue), dx 47, dW 45, the joins 6 and 5 us.
 // Tried and not kept: fragments read a step ahead in a second register set (no change), steps of 128 bytes in two pairs of slots (two
 // workgroups a CU: 60 -> 70 us at K = 256), eight waves on 256 x 128 with a ring of three 128-byte steps (75 us at K = 256, 174 at K = 1024).
 //
@@ -294,6 +294,29 @@ __global__ __launch_bounds__(NT, 2) void gated_dma_kernel(GLArgs p, int tiles_p,
         return v;
     };
 
+    // BWD: dz of 16 pixels at a time in whole rows, one 16-byte load a lane; the first ones under the K loop
+    constexpr int DCH = WTP / 16, DROW = WTP + 16;               // 16-byte chunks of the wave's features in a pixel, bytes of its staging row
+    auto fetch_dz = [&](int j) {
+        u32x4 v = {0, 0, 0, 0};
+        const int64_t m = q0 + wq * WTQ + 16 * j + lane / DCH;
+        const int f = p0 + wp * (WTP / 2) + lane % DCH * 8;
+        if (lane < 16 * DCH && m < p.M && f < p.F) {
+            const bf16_t *src = reinterpret_cast<const bf16_t *>(p.dz) + m * p.lddz + f;
+            if (p.lddz % 8 == 0 && (reinterpret_cast<size_t>(p.dz) & 15) == 0 && f + 8 <= p.F) {
+                v = *reinterpret_cast<const u32x4 *>(src);
+            } else {
+                bf16x8 e = __builtin_bit_cast(bf16x8, v);
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (f + r < p.F) e[r] = src[r];
+                v = __builtin_bit_cast(u32x4, e);
+            }
+        }
+        return v;
+    };
+    u32x4 next_dz;
+    if constexpr (MODE == BWD) next_dz = fetch_dz(0);
+
 #pragma unroll
     for (int h = 0; h < LOOK; ++h) issue(h, h);
     int slot = 0, fill = LOOK;
@@ -405,33 +428,23 @@ __global__ __launch_bounds__(NT, 2) void gated_dma_kernel(GLArgs p, int tiles_p,
                 for (int i = 0; i < MT / 2; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) sg[i][r] = su[i][r] = 0.f;
-                const bool vec = p.lddz % 4 == 0 && (reinterpret_cast<size_t>(p.dz) & (4 * ES - 1)) == 0;
+                static_assert(16 * DCH <= 64 && 4 * 16 * (OROW + DROW) <= RING * SLOT, "one load a lane; both staging tiles live in the ring");
+                unsigned char *Dt = smem + 4 * 16 * OROW + wave * 16 * DROW;
 #pragma unroll
                 for (int j = 0; j < QT; ++j) {
                     const int64_t m = q0 + wq * WTQ + 16 * j + l16;
+                    if (lane < 16 * DCH) *reinterpret_cast<u32x4 *>(Dt + lane / DCH * DROW + lane % DCH * 16) = next_dz;
+                    if (j + 1 < QT) next_dz = fetch_dz(j + 1);
+                    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
                     float w[MT / 2][4];
-                    __builtin_amdgcn_sched_barrier(0);           // (or every j's dz is fetched at once, and the accumulators spill)
 #pragma unroll
                     for (int i = 0; i < MT / 2; ++i) {
                         const int f = fw + 16 * i + q4;
-                        float dz[4] = {0.f, 0.f, 0.f, 0.f}, v[4];
-                        if (m < p.M && f < p.F) {
-                            const T *src = (const T *)p.dz + m * p.lddz + f;
-                            if (vec && f + 3 < p.F) {
-                                if constexpr (ES == 4) {
-                                    const f32x4 t = *reinterpret_cast<const f32x4 *>(src);
+                        const bf16x4 t = *reinterpret_cast<const bf16x4 *>(Dt + l16 * DROW + (16 * i + q4) * 2);
+                        float dz[4], v[4];
 #pragma unroll
-                                    for (int r = 0; r < 4; ++r) dz[r] = t[r];
-                                } else {
-                                    const bf16x4 t = *reinterpret_cast<const bf16x4 *>(src);
-#pragma unroll
-                                    for (int r = 0; r < 4; ++r) dz[r] = f32of<DT>(t[r]);
-                                }
-                            } else {
-                                for (int r = 0; r < 4; ++r)
-                                    if (f + r < p.F) dz[r] = Elem<T>::ld(src + r);
-                            }
-                        }
+                        for (int r = 0; r < 4; ++r) dz[r] = f32of<DT>(t[r]);
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             float a, da;

@@ -157,6 +157,7 @@ def test_c_abi_refusals():
     assert fwd(nr(threshold=-1)) and b'threshold' in err()
     assert fwd(nr(samples=70000)) and b'bad sizes' in err()
     assert fwd(nr(rows=0)) == 0
+    assert lib.rdfc_norm_residual(ctypes.byref(nr()), 16, 16, *[None] * 7, 16, 16, 8, None) and b'aligned' in err()       # stats at 8
     assert lib.rdfc_norm_residual_scratch_floats(ctypes.byref(nr(C=0)), 0) == 0
     bwd = lambda d, lddy=8, lddn=8: lib.rdfc_norm_residual_backward(ctypes.byref(d), *[None] * 9, None, lddy, None, lddn, *[None] * 10)
     assert bwd(nr()) and b'null' in err()
@@ -168,7 +169,10 @@ def test_c_abi_refusals():
     assert fwd(gl(ldwu=4)) and b'ld smaller' in err()
     assert fwd(gl(K=0)) and b'bad sizes' in err()
     assert fwd(gl(F=(1 << 20) + 1)) and b'bad sizes' in err()
+    assert fwd(gl(F=1 << 19, K=1 << 18, ldx=1 << 18, ldwg=1 << 18, ldwu=1 << 18)) and b'too large' in err()
     assert fwd(gl(M=0)) == 0
+    assert lib.rdfc_gated_linear(ctypes.byref(gl()), 16, 16, 16, None, None, None, 16, 16, None) and b'f32 maps' in err()   # pre beside a 16-bit map
+    assert lib.rdfc_gated_linear(ctypes.byref(gl()), 2, 16, 16, None, None, None, 16, None, None) and b'scratch' in err()   # misaligned x, no scratch
     assert lib.rdfc_gated_linear_scratch_bytes(ctypes.byref(gl(dtype=9)), None, None, None, 0) == 0
     assert lib.rdfc_gated_linear_scratch_bytes(ctypes.byref(gl()), 16, 32, 48, 0) == 0
     assert lib.rdfc_gated_linear_scratch_bytes(ctypes.byref(gl()), 2, 32, 48, 0) == 256

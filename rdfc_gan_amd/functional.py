@@ -1146,10 +1146,14 @@ class _NormResidual(torch.autograd.Function):
         d, has_post, has_pre = ctx.meta
         if dy is None and dn is None:
             return (None,) * 13
-        dy, dn = (None if g is None else hip.as_pm(g if g.dtype == x.dtype else g.to(x.dtype)) for g in (dy, dn))
-        grads = hip.norm_residual_backward(d, x, h, gate, scale, (post_w, post_b) if has_post else None, (pre_w, None) if has_pre else None, key, stats,
-                                           dy, dn, ctx.needs_input_grad[2:8])
-        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None, None, None)
+        if dy is not None:
+            dy = hip.as_pm(dy if dy.dtype == x.dtype else dy.to(x.dtype))
+        if dn is not None:
+            dn = hip.as_pm(dn if dn.dtype == x.dtype else dn.to(x.dtype))
+        need = ctx.needs_input_grad
+        dx, dh, *cols = hip.norm_residual_backward(d, x, h, gate, scale, (post_w, post_b) if has_post else None, (pre_w, None) if has_pre else None, key,
+                                                   stats, dy, dn, need[2:8])
+        return (dx if need[0] else None, dh if need[1] else None, *cols, None, None, None, None, None)
 
 
 def _norm_params(wb, what, C, device):

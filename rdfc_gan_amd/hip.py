@@ -1127,19 +1127,26 @@ def norm_residual_backward(d, x, h, gate, scale, post, pre, key, stats, dy, dn, 
     N, H, W, Cc = x.shape
     pw, pb = post or (None, None)
     qw = pre[0] if pre else None
-    dx = torch.empty(N, H, W, Cc, dtype=x.dtype, device=x.device)
-    dh = torch.empty_like(dx) if h is not None else None
+    dev = x.device
+    dx = torch.empty(N, H, W, Cc, dtype=x.dtype, device=dev)
+    dh = torch.empty(N, H, W, Cc, dtype=x.dtype, device=dev) if h is not None else None
     cols, scratch = [None] * 6, None
-    if any(want):
+    if True in want:
         # (the small gradients are slices of one allocation)
-        sizes = [(N if i == 0 else 1) * Cc for i, w in enumerate(want) if w]
-        flat = iter(torch.empty(sum(sizes), dtype=torch.float32, device=x.device).split(sizes))
-        cols = [(next(flat).view(N, Cc) if i == 0 else next(flat)) if w else None for i, w in enumerate(want)]
+        sizes = [Cc] * want.count(True)
+        if want[0]:
+            sizes[0] = N * Cc
+        parts = torch.split_with_sizes(torch.empty(sum(sizes), dtype=torch.float32, device=dev), sizes)
+        at = 0
+        for i, w in enumerate(want):
+            if w:
+                cols[i] = parts[at] if i else parts[0].view(N, Cc)
+                at += 1
         key_ = (d.rows, d.samples, Cc, gate is not None)
         n = _nr_scratch.get(key_)
         if n is None:
             n = _nr_scratch[key_] = lib().rdfc_norm_residual_scratch_floats(C.byref(d), int(gate is not None))
-        scratch = torch.empty(n, dtype=torch.float32, device=x.device)
+        scratch = torch.empty(n, dtype=torch.float32, device=dev)
     _call('rdfc_norm_residual_backward', x, C.byref(d), _a(x), _a(h), _a(gate), _a(scale), _a(pw), _a(pb), _a(qw), _a(key), _a(stats), _a(dy),
           ld(dy) if dy is not None else Cc, _a(dn), ld(dn) if dn is not None else Cc, _a(dx), _a(dh), _a(scratch), *map(_a, cols))
     return (dx, dh, *cols)

@@ -1127,6 +1127,25 @@ def dropout(x, p, training=True, rng=None):
     return _Dropout.apply(x, threshold, seed, offset, key) if threshold else x
 
 
+def _layout_of(*tensors):
+    """(shape, type, device) of the tensors that a forward pass saves"""
+    return [t if t is None else (t.shape, t.dtype, t.device) for t in tensors]
+
+
+def _unpacked(saved, layout, weights=()):
+    """saved tensors as the kernels read them: maps through (pointer, ld), `weights` (positions) as dense rows, the rest dense.  Saved-tensor
+    hooks may return them with other strides than the forward pass had (values moved to the host and back come dense); another shape, type
+    or device is refused."""
+    out = []
+    for i, (t, want) in enumerate(zip(saved, layout)):
+        if t is not None:
+            if (t.shape, t.dtype, t.device) != want:
+                raise RuntimeError(f'a saved-tensor hook returned {tuple(t.shape)} of {t.dtype} on {t.device} for {tuple(want[0])} of {want[1]} on {want[2]}')
+            t = hip.as_pm(t) if t.dim() == 4 else _weight_rows(t, t.dtype) if i in weights else t.contiguous()
+        out.append(t)
+    return out
+
+
 class _NormResidual(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, h, gate, scale, post_w, post_b, pre_w, pre_b, has_post, has_pre, layer, eps, drop):
@@ -1134,16 +1153,17 @@ class _NormResidual(torch.autograd.Function):
         h = hip.as_pm(h) if h is not None else None
         post, pre = (post_w, post_b) if has_post else None, (pre_w, pre_b) if has_pre else None
         d, y, n, stats = hip.norm_residual(x, h, gate, scale, post, pre, layer, eps, *drop, want_stats=any(ctx.needs_input_grad))
-        ctx.save_for_backward(x, h, gate, scale, post_w, post_b, pre_w, stats, drop[3])
-        ctx.meta = d, has_post, has_pre
+        saved = x, h, gate, scale, post_w, post_b, pre_w, stats, drop[3]
+        ctx.save_for_backward(*saved)
+        ctx.meta = d, has_post, has_pre, _layout_of(*saved)
         ctx.set_materialize_grads(False)
         return y, n
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dn):
-        x, h, gate, scale, post_w, post_b, pre_w, stats, key = ctx.saved_tensors
-        d, has_post, has_pre = ctx.meta
+        d, has_post, has_pre, layout = ctx.meta
+        x, h, gate, scale, post_w, post_b, pre_w, stats, key = _unpacked(ctx.saved_tensors, layout)
         if dy is None and dn is None:
             return (None,) * 13
         if dy is not None:
@@ -1220,17 +1240,19 @@ class _GatedLinear(torch.autograd.Function):
         ctx.dw_dtype = wg.dtype
         wg, wu = (_weight_rows(w, x.dtype) for w in (wg, wu))
         d, z, pre = hip.gated_linear(x, wg, wu, bg, bu, act, want_pre=any(ctx.needs_input_grad))
-        ctx.save_for_backward(x, wg, wu, bg, bu, pre)
-        ctx.desc = d
+        saved = x, wg, wu, bg, bu, pre
+        ctx.save_for_backward(*saved)
+        ctx.meta = d, _layout_of(*saved)
         return z
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dz):
-        x, wg, wu, bg, bu, pre = ctx.saved_tensors
+        d, layout = ctx.meta
+        x, wg, wu, bg, bu, pre = _unpacked(ctx.saved_tensors, layout, weights=(1, 2))
         need = ctx.needs_input_grad
         dz = hip.as_pm(dz if dz.dtype == x.dtype else dz.to(x.dtype))
-        grads = hip.gated_linear_backward(ctx.desc, x, wg, wu, bg, bu, pre, dz, need[0], ctx.dw_dtype if need[1] or need[2] else None, need[3] or need[4])
+        grads = hip.gated_linear_backward(d, x, wg, wu, bg, bu, pre, dz, need[0], ctx.dw_dtype if need[1] or need[2] else None, need[3] or need[4])
         return (*(g if n else None for g, n in zip(grads, need)), None)
 
 

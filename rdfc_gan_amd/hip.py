@@ -1123,8 +1123,11 @@ _nr_scratch = {}         # sizes -> floats of scratch
 
 
 def norm_residual_backward(d, x, h, gate, scale, post, pre, key, stats, dy, dn, want):
-    """want: which of (gate, scale, post_w, post_b, pre_w, pre_b) need a gradient -> (dx, dh, those six)"""
+    """d: the forward call's descriptor, whose strides need not be those of x and h here (a saved-tensor hook may return them laid out
+    anew).  want: which of (gate, scale, post_w, post_b, pre_w, pre_b) need a gradient -> (dx, dh, those six)"""
     N, H, W, Cc = x.shape
+    d = NormResidualDesc.from_buffer_copy(d)
+    d.ldx, d.ldh = ld(x), ld(h) if h is not None else Cc
     pw, pb = post or (None, None)
     qw = pre[0] if pre else None
     dev = x.device
@@ -1157,11 +1160,15 @@ def _gated_scratch(d, x, wg, wu, backward):
     return torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
 
 
+def _row_stride(w):
+    return w.stride(0) if w.shape[0] > 1 else w.shape[1]
+
+
 def gated_linear(x, wg, wu, bg, bu, act, want_pre=False):
     """-> (descriptor, z, pre); x pixel-major, weights [F, K] rows of the map's type; want_pre: a backward pass follows (f32 maps keep g and u)"""
     N, H, W, K = x.shape
     F = wg.shape[0]
-    d = GatedDesc(N * H * W, K, F, ld(x), wg.stride(0) if F > 1 else K, wu.stride(0) if F > 1 else K, dt(x), GATE_ACT[act])
+    d = GatedDesc(N * H * W, K, F, ld(x), _row_stride(wg), _row_stride(wu), dt(x), GATE_ACT[act])
     z = torch.empty(N, H, W, F, dtype=x.dtype, device=x.device)
     pre = torch.empty(N * H * W, 2 * ((F + 31) // 32 * 32), dtype=torch.float32, device=x.device) if want_pre and x.dtype == torch.float32 else None
     if z.numel():
@@ -1171,9 +1178,12 @@ def gated_linear(x, wg, wu, bg, bu, act, want_pre=False):
 
 
 def gated_linear_backward(d, x, wg, wu, bg, bu, pre, dz, want_dx, dw_dtype, want_bias):
-    """dw_dtype: None (no weight gradients), f32 or the map's type -> (dx, dwg, dwu, dbg, dbu)"""
+    """d: the forward call's descriptor, whose strides need not be those of the operands here (a saved-tensor hook may return them laid
+    out anew).  dw_dtype: None (no weight gradients), f32 or the map's type -> (dx, dwg, dwu, dbg, dbu)"""
     N, H, W, K = x.shape
     F = wg.shape[0]
+    d = GatedDesc.from_buffer_copy(d)
+    d.ldx, d.ldwg, d.ldwu = ld(x), _row_stride(wg), _row_stride(wu)
     dx = torch.empty(N, H, W, K, dtype=x.dtype, device=x.device) if want_dx else None
     dwg, dwu = (torch.empty(F, K, dtype=dw_dtype, device=x.device) for _ in range(2)) if dw_dtype is not None else (None, None)
     dbg, dbu = (torch.empty(F, dtype=torch.float32, device=x.device) for _ in range(2)) if want_bias else (None, None)

@@ -182,6 +182,64 @@ def test_c_abi_refusals():
     assert bwd(gl(), dw=2) and b'weight gradients' in err()
 
 
+# ---- what reaches the C ABI: the entry points are recorded, not called -----------------------------------------------------
+@pytest.fixture
+def calls(monkeypatch):
+    from rdfc_gan_amd import functional as Fh
+    from rdfc_gan_amd import hip
+    seen = []
+
+    def record(name, t, *args):
+        d = args[0]._obj if hasattr(args[0], '_obj') else None
+        seen.append((name, {k: getattr(d, k) for k, _ in d._fields_} if d is not None else None, args))
+    monkeypatch.setattr(hip, '_call', record)
+    monkeypatch.setattr(Fh, '_check_device', lambda t, what: None)
+    return seen
+
+
+def _slice(shape, lead, tail):
+    wide = torch.zeros(*shape[:-1], lead + shape[-1] + tail)
+    return wide[..., lead:lead + shape[-1]]
+
+
+# what a saved-tensor hook may do to strides: everything dense (as moving it to the host and back does), or everything a slice of something wider
+RELAY = {'dense': lambda t: t.clone(memory_format=torch.contiguous_format), 'wide': lambda t: _slice(t.shape, 8, 5).copy_(t)}
+
+
+@pytest.mark.parametrize('relay', list(RELAY))
+def test_backward_passes_take_the_strides_of_what_hooks_return(calls, relay):
+    """the strides that a backward pass hands to its kernels are those of the tensors it reads, not those of the forward call"""
+    from rdfc_gan_amd import functional as Fh
+    x, h = (_slice((2, 3, 5, 67), 3, 61).requires_grad_(True) for _ in range(2))
+    gate, w = torch.ones(2, 67, requires_grad=True), torch.ones(67, requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(RELAY[relay], lambda t: t):
+        y, n = Fh.norm_residual(x, h, gate=gate, post=(w, None), pre=(w, None))
+    torch.autograd.grad([y, n], [x, gate], [torch.zeros_like(y)] * 2)
+    (_, fwd, _), (name, bwd, args) = calls
+    assert fwd['ldx'] == fwd['ldh'] == 131 and name == 'rdfc_norm_residual_backward'
+    assert bwd['ldx'] == bwd['ldh'] == {'dense': 67, 'wide': 80}[relay]
+    calls.clear()
+    wg, wu = (_slice((40, 67), 3, 61).requires_grad_(True) for _ in range(2))
+    with torch.autograd.graph.saved_tensors_hooks(RELAY[relay], lambda t: t):
+        z = Fh.gated_linear(x, wg, wu)
+    torch.autograd.grad(z, [x, wg], torch.zeros_like(z))
+    (_, fwd, _), (name, bwd, args) = calls
+    assert [fwd[k] for k in ('ldx', 'ldwg', 'ldwu')] == [131] * 3 and name == 'rdfc_gated_linear_backward'
+    assert [bwd[k] for k in ('ldx', 'ldwg', 'ldwu')] == [{'dense': 67, 'wide': 80}[relay]] * 3
+
+
+@pytest.mark.parametrize('wrong', [lambda t: t.double() if t.is_floating_point() else t, lambda t: t[:1] if t.dim() == 4 else t], ids=['type', 'shape'])
+def test_backward_passes_refuse_other_values_from_hooks(calls, wrong):
+    from rdfc_gan_amd import functional as Fh
+    x = torch.zeros(2, 3, 5, 8, requires_grad=True)
+    w = torch.zeros(4, 8, requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, wrong):
+        outs = Fh.row_norm(x), Fh.gated_linear(x, w, w)
+    for o in outs:
+        with pytest.raises(RuntimeError, match='saved-tensor hook'):
+            torch.autograd.grad(o, x, torch.zeros_like(o))
+
+
 def test_residual_block_with_dropout_has_upstream_indices():
     """use_dropout puts nn.Dropout(0.5) behind the first activation: the second convolution is conv_block.6"""
     from rdfc_gan_amd.generator import ResnetGenerator

@@ -523,6 +523,31 @@ def test_gated_linear_is_reproducible_and_takes_two_streams():
             assert torch.equal(p, q)
 
 
+def test_gradients_through_saved_tensor_hooks():
+    """channel slices whose saved copies come back dense, from the host, or inside a wider buffer: the gradients of a run without hooks, bit for bit"""
+    def wider(t):
+        wide = torch.full((*t.shape[:-1], t.shape[-1] + 13), 7.0, dtype=torch.float64, device=DEV).to(t.dtype)
+        wide[..., 8:8 + t.shape[-1]] = t
+        return wide[..., 8:8 + t.shape[-1]]
+    relays = [(lambda t: t, lambda t: t), (lambda t: t.clone(memory_format=torch.contiguous_format), lambda t: t),
+              (lambda t: t.cpu(), lambda t: t.to(DEV)), (lambda t: wider(t) if t.dim() > 1 and t.is_floating_point() else t, lambda t: t)]
+    for dtype in DTYPES:
+        x, h, gy, gn = (lay(rnd(2, 3, 5, 67, seed=i, dtype=dtype), 'slice').requires_grad_(i < 2) for i in range(4))
+        gate, w = (rnd(*s, seed=6, mean=1.0).to(DEV).requires_grad_(True) for s in ((2, 67), (67,)))
+        wide = rnd(80, 131, seed=7, std=0.1, dtype=dtype).to(DEV)
+        wg, wu = (wide[40 * i:40 * i + 40, 3:70].detach().requires_grad_(True) for i in range(2))
+        gz = rnd(2, 3, 5, 40, seed=8, dtype=dtype).to(DEV)
+        want = None
+        for pack, unpack in relays:
+            with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+                y, n = Fh().norm_residual(x, h, gate=gate, post=(w, None), pre=(w, None), p=0.2, rng=(3, 4))
+                z = Fh().gated_linear(x, wg, wu)
+            got = torch.autograd.grad([y, n], [x, h, gate, w], [gy, gn]) + torch.autograd.grad(z, [x, wg, wu], gz)
+            want = want or got
+            for i, (a, b) in enumerate(zip(got, want)):
+                assert torch.equal(a, b), (dtype, i)
+
+
 # ---- together -------------------------------------------------------------------------------------------------------------
 def plain_trunk(trunk, x, gate, keeps):
     """the trunk in f64 from its parameters; keeps: dropout factors per block"""

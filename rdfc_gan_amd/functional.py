@@ -1028,10 +1028,12 @@ def normal_losses(normal, gt_normal, norm_mask, logits_nchw, label_wall, label_f
 # ---- operators of transformer blocks on pixel-major maps (a pixel is a token) ----------------------------------------------------
 class DropoutState:
     """Generator state {seed, counter} in device memory.  Every draw copies it into a key of its own and advances the counter, on the
-    current stream: a captured HIP graph draws new masks at every replay, and a backward pass reads its own forward's key."""
+    current stream: a captured HIP graph draws new masks at every replay, and a backward pass reads its own forward's key.  Without a seed
+    one is drawn from torch's CPU generator: states made one after the other draw different masks, and torch.manual_seed repeats
+    them.  Two states of the same seed draw the same masks."""
 
     def __init__(self, seed=None, device='cuda'):
-        seed = torch.initial_seed() if seed is None else int(seed)
+        seed = int(torch.empty((), dtype=torch.int64, device='cpu').random_()) if seed is None else int(seed)
         self.state = torch.tensor([_signed64(seed), 0], dtype=torch.int64, device=device)
 
     def draw(self):

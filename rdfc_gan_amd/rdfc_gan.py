@@ -728,11 +728,24 @@ class RDFCGAN:
         if enabled:
             for o in self.optimizers.values():
                 o.make_capturable()
-            # (elementwise dropout inside a captured step draws from a state in device memory: every replay its own masks)
-            for net in (self.G_A2B, self.G_B2A):
-                for m in net.modules():
-                    if isinstance(m, layers.Dropout) and m.rng is None:
-                        m.rng = Fh.DropoutState(device=self.device)
+        self._graph_dropout(enabled)
+
+    def _graph_dropout(self, enabled):
+        """elementwise dropout inside a captured step draws from a state in device memory, every replay its own masks and every layer from
+        a state (a seed) of its own; outside graph mode the layers draw from torch's generator again.  A layer whose rng the caller
+        has set keeps it."""
+        states = self.__dict__.setdefault('_dropout_states', {})
+        for key in ('G_A2B', 'G_B2A'):
+            for name, m in getattr(self, key).named_modules():
+                if not isinstance(m, (layers.Dropout, layers.GatedFeedForward)):
+                    continue
+                name = f'{key}.{name}'
+                if enabled and m.rng is None:
+                    if name not in states:
+                        states[name] = Fh.DropoutState(device=self.device)
+                    m.rng = states[name]
+                elif not enabled and name in states and m.rng is states[name]:
+                    m.rng = None
 
     def _mask_to_device(self, mask):
         """host mask -> device through a pinned staging buffer: a pageable-memory copy makes the host wait for every kernel
@@ -850,6 +863,7 @@ class RDFCGAN:
                 warnings.warn(f'HIP graph capture failed ({type(e).__name__}: {e}); continuing with eager launches')
                 torch.cuda.synchronize()
                 self._graph_mode, self._graphs = False, None
+                self._graph_dropout(False)
                 self.set_input(self._batch)
                 return self.optimize_parameters(sync_losses)
         g1, g2, g3, stats = self._graphs

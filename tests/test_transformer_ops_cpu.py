@@ -248,3 +248,41 @@ def test_residual_block_with_dropout_has_upstream_indices():
     assert {k.split('conv_block.')[1] for k in keys} == {'1.weight', '1.bias', '6.weight', '6.bias'}
     plain = ResnetGenerator(1, 3, ngf=8, norm_layer='IN2d', n_blocks=1)
     assert {k.split('conv_block.')[1] for k in plain.state_dict() if 'conv_block' in k} == {'1.weight', '1.bias', '5.weight', '5.bias'}
+
+
+def test_unseeded_states_are_streams_of_their_own():
+    from rdfc_gan_amd.functional import DropoutState
+    torch.manual_seed(5)
+    a, b = (DropoutState(device='cpu').state.clone() for _ in range(2))
+    torch.manual_seed(5)
+    c, d = (DropoutState(device='cpu').state.clone() for _ in range(2))
+    assert torch.equal(a, c) and torch.equal(b, d) and int(a[0]) != int(b[0]) and int(a[1]) == int(b[1]) == 0
+    assert torch.equal(DropoutState(7, 'cpu').state, DropoutState(7, 'cpu').state)
+
+
+def _graph_model():
+    """what enable_graph needs of an RDFCGAN: two generators, one with dropout, no optimizers"""
+    from rdfc_gan_amd.generator import ResnetGenerator
+    from rdfc_gan_amd.rdfc_gan import RDFCGAN
+    m = RDFCGAN.__new__(RDFCGAN)
+    m.use_label_net, m.G_normal, m.optimizers, m.device = False, None, {}, torch.device('cpu')
+    m.G_A2B = ResnetGenerator(1, 3, ngf=8, norm_layer='IN2d', n_blocks=1)
+    m.G_B2A = ResnetGenerator(1, 3, ngf=8, norm_layer='IN2d', use_dropout=True, n_blocks=4)
+    return m, [d for d in m.G_B2A.modules() if isinstance(d, torch.nn.Dropout)]
+
+
+def test_graph_mode_gives_every_dropout_layer_a_state_of_its_own():
+    from rdfc_gan_amd import functional as Fh
+    many = Fh.multi_stream()
+    try:
+        m, drops = _graph_model()
+        own = drops[0].rng = (1, 2)
+        m.enable_graph(True)
+        states = [d.rng for d in drops[1:]]
+        assert drops[0].rng is own and len({int(s.state[0]) for s in states}) == 3
+        m.enable_graph(False)                            # eager steps follow torch's generator again
+        assert drops[0].rng is own and all(d.rng is None for d in drops[1:])
+        m.enable_graph(True)                             # and graph mode goes on where it was
+        assert [d.rng for d in drops[1:]] == states
+    finally:
+        Fh.set_multi_stream(many)

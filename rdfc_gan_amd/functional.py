@@ -1149,12 +1149,14 @@ def _unpacked(saved, layout, weights=()):
 
 
 class _NormResidual(torch.autograd.Function):
+    # grad_on: the caller's grad mode.  It is off inside forward, and needs_input_grad does not know it: without it a no_grad call would
+    # write what only a backward pass reads
     @staticmethod
-    def forward(ctx, x, h, gate, scale, post_w, post_b, pre_w, pre_b, has_post, has_pre, layer, eps, drop):
+    def forward(ctx, x, h, gate, scale, post_w, post_b, pre_w, pre_b, has_post, has_pre, layer, eps, drop, grad_on):
         x = hip.as_pm(x)
         h = hip.as_pm(h) if h is not None else None
         post, pre = (post_w, post_b) if has_post else None, (pre_w, pre_b) if has_pre else None
-        d, y, n, stats = hip.norm_residual(x, h, gate, scale, post, pre, layer, eps, *drop, want_stats=any(ctx.needs_input_grad))
+        d, y, n, stats = hip.norm_residual(x, h, gate, scale, post, pre, layer, eps, *drop, want_stats=grad_on and any(ctx.needs_input_grad))
         saved = x, h, gate, scale, post_w, post_b, pre_w, stats, drop[3]
         ctx.save_for_backward(*saved)
         ctx.meta = d, has_post, has_pre, _layout_of(*saved)
@@ -1167,7 +1169,7 @@ class _NormResidual(torch.autograd.Function):
         d, has_post, has_pre, layout = ctx.meta
         x, h, gate, scale, post_w, post_b, pre_w, stats, key = _unpacked(ctx.saved_tensors, layout)
         if dy is None and dn is None:
-            return (None,) * 13
+            return (None,) * 14
         if dy is not None:
             dy = hip.as_pm(dy if dy.dtype == x.dtype else dy.to(x.dtype))
         if dn is not None:
@@ -1175,7 +1177,7 @@ class _NormResidual(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx, dh, *cols = hip.norm_residual_backward(d, x, h, gate, scale, (post_w, post_b) if has_post else None, (pre_w, None) if has_pre else None, key,
                                                    stats, dy, dn, need[2:8])
-        return (dx if need[0] else None, dh if need[1] else None, *cols, None, None, None, None, None)
+        return (dx if need[0] else None, dh if need[1] else None, *cols, None, None, None, None, None, None)
 
 
 def _norm_params(wb, what, C, device):
@@ -1220,7 +1222,7 @@ def norm_residual(x, h, *, gate=None, scale=None, post=None, pre=None, norm='rms
     has_pre, pre_w, pre_b = _norm_params(pre, 'pre', C, x.device)
     drop = _drop_rng(p, training, rng, x)
     _check_device(x, 'norm_residual')
-    return _NormResidual.apply(x, h, gate, scale, post_w, post_b, pre_w, pre_b, has_post, has_pre, layer, float(eps), drop)
+    return _NormResidual.apply(x, h, gate, scale, post_w, post_b, pre_w, pre_b, has_post, has_pre, layer, float(eps), drop, torch.is_grad_enabled())
 
 
 def row_norm(x, weight=None, bias=None, norm='rms', eps=1e-5):
@@ -1232,16 +1234,16 @@ def row_norm(x, weight=None, bias=None, norm='rms', eps=1e-5):
         raise ValueError(f'row_norm: {C} channels, at most 8192')
     _, w, b = _norm_params((weight, bias), 'row_norm', C, x.device)
     _check_device(x, 'row_norm')
-    return _NormResidual.apply(x, None, None, None, None, None, w, b, False, True, layer, float(eps), (0, 0, 0, None))[1]
+    return _NormResidual.apply(x, None, None, None, None, None, w, b, False, True, layer, float(eps), (0, 0, 0, None), torch.is_grad_enabled())[1]
 
 
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, wg, wu, bg, bu, act):
+    def forward(ctx, x, wg, wu, bg, bu, act, grad_on):
         x = hip.as_pm(x)
         ctx.dw_dtype = wg.dtype
         wg, wu = (_weight_rows(w, x.dtype) for w in (wg, wu))
-        d, z, pre = hip.gated_linear(x, wg, wu, bg, bu, act, want_pre=any(ctx.needs_input_grad))
+        d, z, pre = hip.gated_linear(x, wg, wu, bg, bu, act, want_pre=grad_on and any(ctx.needs_input_grad))
         saved = x, wg, wu, bg, bu, pre
         ctx.save_for_backward(*saved)
         ctx.meta = d, _layout_of(*saved)
@@ -1255,7 +1257,7 @@ class _GatedLinear(torch.autograd.Function):
         need = ctx.needs_input_grad
         dz = hip.as_pm(dz if dz.dtype == x.dtype else dz.to(x.dtype))
         grads = hip.gated_linear_backward(d, x, wg, wu, bg, bu, pre, dz, need[0], ctx.dw_dtype if need[1] or need[2] else None, need[3] or need[4])
-        return (*(g if n else None for g, n in zip(grads, need)), None)
+        return (*(g if n else None for g, n in zip(grads, need)), None, None)
 
 
 def _weight_rows(w, dtype):
@@ -1288,4 +1290,4 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act='silu'):
         raise ValueError('gated_linear: one bias without the other')
     b_gate, b_up = _check_param(b_gate, 'b_gate', (F,), x.device), _check_param(b_up, 'b_up', (F,), x.device)
     _check_device(x, 'gated_linear')
-    return _GatedLinear.apply(x, w_gate, w_up, b_gate, b_up, act)
+    return _GatedLinear.apply(x, w_gate, w_up, b_gate, b_up, act, torch.is_grad_enabled())

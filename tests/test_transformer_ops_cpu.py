@@ -240,6 +240,26 @@ def test_backward_passes_refuse_other_values_from_hooks(calls, wrong):
             torch.autograd.grad(o, x, torch.zeros_like(o))
 
 
+def test_calls_that_no_backward_pass_can_follow_keep_nothing_for_one(calls):
+    """parameters under no_grad or inference_mode, and plain tensors: no statistics, no kept projections; with grad mode on: both"""
+    from rdfc_gan_amd import functional as Fh
+    x, plain = torch.zeros(2, 3, 5, 8), torch.ones(8)
+    w, m = torch.nn.Parameter(torch.ones(8)), torch.nn.Parameter(torch.zeros(4, 8))
+
+    def kept():
+        calls.clear()
+        Fh.norm_residual(x, x, post=(w, None), pre=(w, None))
+        Fh.row_norm(x, w)
+        Fh.gated_linear(x, m, m)
+        return [args[-1] for _, _, args in calls]            # (the last argument of either entry point: stats, pre)
+    assert None not in kept()
+    for off in (torch.no_grad, torch.inference_mode):
+        with off():
+            assert kept() == [None] * 3
+    w, m = plain, m.detach()
+    assert kept() == [None] * 3
+
+
 def test_residual_block_with_dropout_has_upstream_indices():
     """use_dropout puts nn.Dropout(0.5) behind the first activation: the second convolution is conv_block.6"""
     from rdfc_gan_amd.generator import ResnetGenerator

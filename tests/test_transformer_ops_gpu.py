@@ -523,6 +523,27 @@ def test_gated_linear_is_reproducible_and_takes_two_streams():
             assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+def test_no_grad_gives_the_same_values_without_what_a_backward_pass_needs(dtype):
+    """parameters under no_grad and inference_mode: the outputs of a training call, and no memory beyond them"""
+    x, h = rnd(2, 29, 38, 64, seed=1, dtype=dtype).to(DEV), rnd(2, 29, 38, 64, seed=2, dtype=dtype).to(DEV)
+    w = torch.nn.Parameter(rnd(64, seed=3, mean=1.0).to(DEV))
+    m = [torch.nn.Parameter(rnd(256, 64, seed=4 + i, std=0.1, dtype=dtype).to(DEV)) for i in range(2)]
+
+    def run():
+        return [*Fh().norm_residual(x, h, post=(w, None), pre=(w, None)), Fh().row_norm(x, w), Fh().gated_linear(x, *m)]
+    want = run()
+    for off in (torch.no_grad, torch.inference_mode):
+        with off():
+            torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
+            before = torch.cuda.memory_stats()['requested_bytes.all.current']
+            got = run()
+            grown = torch.cuda.memory_stats()['requested_bytes.all.peak'] - before
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert grown == sum(t.numel() * t.element_size() for t in got)
+
+
 def test_gradients_through_saved_tensor_hooks():
     """channel slices whose saved copies come back dense, from the host, or inside a wider buffer: the gradients of a run without hooks, bit for bit"""
     def wider(t):

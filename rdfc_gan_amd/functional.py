@@ -16,7 +16,6 @@ Blocks
 """
 import math
 import os
-import threading
 import weakref
 
 import torch
@@ -1040,9 +1039,6 @@ class DropoutState:
         return hip.dropout_draw(self.state)
 
 
-_generator_lock = threading.Lock()
-
-
 def _signed64(v):
     v &= 0xffffffffffffffff
     return v - (1 << 64) if v >> 63 else v
@@ -1070,11 +1066,9 @@ def _drop_rng(p, training, rng, x):
     _check_device(x, 'dropout')
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError('dropout inside a HIP graph: pass rng=DropoutState(...) (torch\'s generator would give every replay the same mask)')
-    gen = torch.cuda.default_generators[device.index]
-    with _generator_lock:
-        at = gen.get_offset()
-        gen.set_offset(at + 4)
-    return threshold, gen.initial_seed() & 0xffffffffffffffff, 1 << 63 | at, None        # (bit 63: apart from the counters of torch's own kernels)
+    # (a key of 126 random bits by one torch call: torch advances its generator under a lock of its own, which no pair of get_offset and
+    # set_offset could take -- a torch kernel launched by another thread between the two would have had its advance undone)
+    return threshold, 0, 0, torch.empty(2, dtype=torch.int64, device=device).random_()
 
 
 def _check_map(t, what, like=None):
@@ -1122,8 +1116,8 @@ class _Dropout(torch.autograd.Function):
 def dropout(x, p, training=True, rng=None):
     """nn.Dropout on a pixel-major map: an element is zeroed with probability T / 65536, T = round(65536 p), the others are scaled by
     1 / (1 - T / 65536).  The mask is a function of (seed, offset, element) -- Philox4x32-10, csrc/philox.h -- and is drawn again by the
-    backward pass, not stored.  rng: None (torch's generator of the device: its seed, and an offset that every call advances by 4), a pair
-    (seed, offset), or a DropoutState (needed inside a captured graph)."""
+    backward pass, not stored.  rng: None (a key drawn from torch's generator of the device, which that advances by 4), a pair (seed, offset), or a
+    DropoutState (needed inside a captured graph)."""
     _check_map(x, 'dropout')
     threshold, seed, offset, key = _drop_rng(p, training, rng, x)
     return _Dropout.apply(x, threshold, seed, offset, key) if threshold else x

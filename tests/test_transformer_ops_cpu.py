@@ -260,6 +260,26 @@ def test_calls_that_no_backward_pass_can_follow_keep_nothing_for_one(calls):
     assert kept() == [None] * 3
 
 
+def test_dropout_draws_from_torchs_generator_through_torch(calls, monkeypatch):
+    """a key drawn by a torch call: nothing sets the generator's offset, where a draw of another thread could be undone"""
+    from rdfc_gan_amd import functional as Fh
+
+    class Untouched:
+        def __getattr__(self, name):
+            raise AssertionError(f'{name} of a generator')
+    monkeypatch.setattr(torch.cuda, 'default_generators', [Untouched()] * 8)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
+    x, keys = torch.zeros(1, 2, 3, 8), []
+    drop = Fh.hip.dropout
+    monkeypatch.setattr(Fh.hip, 'dropout', lambda x, t, seed, offset, key: keys.append(key.clone()) or drop(x, t, seed, offset, key))
+    for _ in range(2):
+        torch.manual_seed(3)
+        Fh.dropout(x, 0.5)
+        Fh.dropout(x, 0.5)
+    assert torch.equal(keys[0], keys[2]) and torch.equal(keys[1], keys[3]) and not torch.equal(keys[0], keys[1])
+    assert all(k.dtype == torch.int64 and k.shape == (2,) for k in keys)
+
+
 def test_residual_block_with_dropout_has_upstream_indices():
     """use_dropout puts nn.Dropout(0.5) behind the first activation: the second convolution is conv_block.6"""
     from rdfc_gan_amd.generator import ResnetGenerator

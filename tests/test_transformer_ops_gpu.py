@@ -125,6 +125,29 @@ def test_dropout_from_several_threads():
     assert len(out) == 80 and len(masks) == 80
 
 
+def test_dropout_beside_torchs_own_draws():
+    """dropout and torch's random kernels from two threads: the generator has advanced by the draws of both, four each, and none is lost"""
+    import threading
+    x = torch.ones(1, 1, 1, 64, device=DEV)
+    n, start = 1500, threading.Barrier(2)
+
+    def work(draw):
+        start.wait()
+        for _ in range(n):
+            draw()
+    torch.manual_seed(12)
+    torch.cuda.synchronize()
+    gen = torch.cuda.default_generators[torch.cuda.current_device()]
+    first = gen.get_offset()
+    threads = [threading.Thread(target=work, args=(f,)) for f in (lambda: Fh().dropout(x, 0.5), lambda: torch.rand(64, device=DEV))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert gen.get_offset() - first == 2 * n * 4
+
+
 def test_dropout_empty_map():
     x = torch.zeros(0, 3, 4, 8, device=DEV, requires_grad=True)
     y = Fh().dropout(x, 0.5, rng=(1, 2))

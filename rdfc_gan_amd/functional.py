@@ -1038,6 +1038,14 @@ class DropoutState:
     def draw(self):
         return hip.dropout_draw(self.state)
 
+    def state_dict(self):
+        seed, counter = self.state.tolist()
+        return dict(seed=seed, counter=counter)
+
+    def load_state_dict(self, sd):
+        """in place: a captured graph that draws from this state goes on from the loaded counter"""
+        self.state.copy_(torch.tensor([sd['seed'], sd['counter']], dtype=torch.int64))
+
 
 def _signed64(v):
     v &= 0xffffffffffffffff

@@ -735,17 +735,38 @@ class RDFCGAN:
         a state (a seed) of its own; outside graph mode the layers draw from torch's generator again.  A layer whose rng the caller
         has set keeps it."""
         states = self.__dict__.setdefault('_dropout_states', {})
+        for name, m in self._dropout_layers():
+            if enabled and m.rng is None:
+                if name not in states:
+                    states[name] = Fh.DropoutState(device=self.device)
+                m.rng = states[name]
+            elif not enabled and name in states and m.rng is states[name]:
+                m.rng = None
+
+    def _dropout_layers(self):
         for key in ('G_A2B', 'G_B2A'):
             for name, m in getattr(self, key).named_modules():
-                if not isinstance(m, (layers.Dropout, layers.GatedFeedForward)):
-                    continue
-                name = f'{key}.{name}'
-                if enabled and m.rng is None:
-                    if name not in states:
-                        states[name] = Fh.DropoutState(device=self.device)
-                    m.rng = states[name]
-                elif not enabled and name in states and m.rng is states[name]:
-                    m.rng = None
+                if isinstance(m, (layers.Dropout, layers.GatedFeedForward)):
+                    yield f'{key}.{name}', m
+
+    def _dropout_state_dict(self):
+        """the DropoutStates that graph mode (in use or not) or the caller has given to layers, by the layer's name"""
+        states = dict(self.__dict__.get('_dropout_states', {}))
+        states.update((name, m.rng) for name, m in self._dropout_layers() if isinstance(m.rng, Fh.DropoutState))
+        return {name: s.state_dict() for name, s in states.items()}
+
+    def _load_dropout_state_dict(self, sd):
+        states = self.__dict__.setdefault('_dropout_states', {})
+        layer = dict(self._dropout_layers())
+        other = dist.is_available() and dist.is_initialized() and dist.get_rank() != 0
+        for name, values in sd.items():
+            if name not in layer:
+                continue
+            s = layer[name].rng
+            if not isinstance(s, Fh.DropoutState):       # (for the next enable_graph)
+                s = states[name] if name in states else states.setdefault(name, Fh.DropoutState(device=self.device))
+            # (a checkpoint is one rank's: the others keep their own seeds)
+            s.load_state_dict(dict(values, seed=s.state_dict()['seed']) if other else values)
 
     def _mask_to_device(self, mask):
         """host mask -> device through a pinned staging buffer: a pageable-memory copy makes the host wait for every kernel
@@ -1004,6 +1025,9 @@ class RDFCGAN:
                 ckpt[f'{name}_lr_scheduler_state_dict'] = s.state_dict()
             if self.scaler is not None:           # (a key of its own: upstream-format checkpoints simply do not have it)
                 ckpt['loss_scaler_state_dict'] = self.scaler.state_dict()
+            drops = self._dropout_state_dict()
+            if drops:                             # (likewise)
+                ckpt['dropout_state_dict'] = drops
         torch.save(ckpt, filename)
 
     def load_from(self, load_path, strict=False):
@@ -1025,6 +1049,7 @@ class RDFCGAN:
                 s.load_state_dict(ckpt[f'{name}_lr_scheduler_state_dict'])
         if self.scaler is not None and 'loss_scaler_state_dict' in ckpt:
             self.scaler.load_state_dict(ckpt['loss_scaler_state_dict'])
+        self._load_dropout_state_dict(ckpt.get('dropout_state_dict', {}))
         return ckpt['meta'].get('epoch', 0)
 
     def save_samples(self, save_dir, iters):

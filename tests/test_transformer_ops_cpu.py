@@ -326,3 +326,47 @@ def test_graph_mode_gives_every_dropout_layer_a_state_of_its_own():
         assert [d.rng for d in drops[1:]] == states
     finally:
         Fh.set_multi_stream(many)
+
+
+def test_dropout_states_are_in_the_checkpoint(tmp_path, monkeypatch):
+    """a resumed run goes on with the masks that come next, whether graph mode is on before the checkpoint is read or only afterwards"""
+    from rdfc_gan_amd import functional as Fh
+    many = Fh.multi_stream()
+
+    def model():
+        m, drops = _graph_model()
+        m.is_train, m.scaler, m.lr_schedulers, m.models = True, None, {}, {}
+        return m, drops
+    try:
+        m, drops = model()
+        m.save_ckpt(tmp_path / 'none.pth')
+        assert 'dropout_state_dict' not in torch.load(tmp_path / 'none.pth')
+        drops[0].rng = Fh.DropoutState((1 << 64) - 3, 'cpu')                  # the caller's own; draws: counters move
+        m.enable_graph(True)
+        for i, d in enumerate(drops):
+            d.rng.state[1] += 10 + i
+        want = [d.rng.state.clone() for d in drops]
+        m.save_ckpt(tmp_path / 'a.pth')
+        for early in (True, False):
+            r, drops = model()
+            if early:
+                r.enable_graph(True)
+                held = [d.rng.state for d in drops]
+            r.resume_from(tmp_path / 'a.pth')
+            assert early or all(d.rng is None for d in drops)
+            r.enable_graph(True)
+            assert all(torch.equal(d.rng.state, w) for d, w in zip(drops, want))
+            assert not early or all(d.rng.state is h for d, h in zip(drops, held))        # (in place: a captured step reads it there)
+        with monkeypatch.context() as mp:                # another rank reading rank 0's file: the counters, its own seeds
+            mp.setattr(torch.distributed, 'is_initialized', lambda: True)
+            mp.setattr(torch.distributed, 'get_rank', lambda: 1)
+            o, drops = model()
+            o.enable_graph(True)
+            seeds = [int(d.rng.state[0]) for d in drops]
+            o.resume_from(tmp_path / 'a.pth')
+            assert [d.rng.state.tolist() for d in drops] == [[s, int(w[1])] for s, w in zip(seeds, want)]
+        r.enable_graph(False)
+        r.save_ckpt(tmp_path / 'b.pth')                  # (graph mode is off, its states are kept)
+        assert torch.load(tmp_path / 'b.pth')['dropout_state_dict'] == torch.load(tmp_path / 'a.pth')['dropout_state_dict']
+    finally:
+        Fh.set_multi_stream(many)

@@ -499,6 +499,31 @@ def test_gated_linear_extreme_gates():
             assert bool(torch.isfinite(z).all()) and bool(torch.isfinite(gx).all()), (act, dtype)
 
 
+@pytest.mark.parametrize('dtype,far,up', [(torch.bfloat16, -12.0, 1.0), (torch.float16, -6.0, 32768.0)], ids=IDS[1:])
+def test_gated_linear_gelu_tail_is_relatively_accurate(dtype, far, up):
+    """gates from 0 far into the negative tail, alone in their dot products, so that gelu(g) and its derivative come out scaled by a power of two and normal
+    numbers of the type: relative errors of half a step of the type a rounding (z: one; dx: dg and dx), and 2^-15 for the f32 arithmetic: the fit of
+    phi and the rounding of the exponential's argument (g^2 / 2 half steps of f32 at most 72, 4.3e-6 each of them) are 1.1e-5, twice that where the
+    derivative's two terms partly cancel.  (Left out: around the derivative's zero at -0.7518, where the terms cancel altogether.)"""
+    import math
+    half = torch.finfo(dtype).eps / 2
+    g = torch.linspace(0.0, far, 3001).to(dtype).unique()
+    x = torch.stack([g, torch.ones_like(g)], 1).view(1, 1, -1, 2).to(DEV).requires_grad_(True)
+    wg, wu = (torch.tensor([row], dtype=dtype, device=DEV).expand(8, 2).contiguous() for row in ([1.0, 0.0], [0.0, up]))
+    z = Fh().gated_linear(x, wg, wu, act='gelu')
+    dz = torch.zeros_like(z)
+    dz[..., 3] = 1.0
+    dx, = torch.autograd.grad(z, x, dz)
+    g = g.double()
+    phi, pdf = 0.5 * torch.special.erfc(-g * math.sqrt(0.5)), torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+    for got, want, steps in ((z[0, 0, :, 3], g * phi * up, 1), (dx[0, 0, :, 0], (phi + g * pdf) * up, 2)):
+        got, use = got.detach().double().cpu(), torch.ones_like(g, dtype=torch.bool) if steps == 1 else (g < -1.2) | (g > -0.4)
+        off = (got - want).abs() - (2.0 ** -25 if dtype == torch.float16 else 0.0) * steps
+        rel = (off / want.abs())[use & (want != 0)]
+        worst = float(rel.max())
+        assert worst <= steps * half * (1 + half) + 2.0 ** -15, (steps, worst)
+
+
 def test_gated_linear_keeps_nan_rows_apart():
     """a NaN or infinite pixel spoils its own row only"""
     for M, K, F in ((5, 64, 40), (150, 72, 136), (300, 40, 264)):

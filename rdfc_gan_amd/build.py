@@ -15,19 +15,10 @@ CSRC = os.path.join(HERE, 'csrc')
 OBJ = os.path.join(CSRC, 'build')
 LIB = os.path.join(HERE, 'librdfc_hip.so')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
-FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fno-gpu-rdc', '-Wno-unused-value',
-         '-Wno-pass-failed']
 # hipcc makes packed f32 instructions of ordinary float code by itself, and some of their forms have given wrong results on gfx950 now and
-# then: they are switched off (hipcc's host pass does not know the feature and says so: harmless).  The sources in KEEPS_PACKED are older than
-# that and stay as they were built: without packed instructions hipcc fuses other multiplications and additions there, results move in the
-# last bits, and one fixture's LeakyReLU takes its other side (tests/test_normal_net_gpu.py, f32).  In every other source the fused
-# operations are the same ones either way.
-NO_PACKED = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
-KEEPS_PACKED = ('conv_glds.hip', 'label_ops.hip', 'mdconv.hip', 'nlspn.hip', 'norm.hip', 'pointwise.hip')
-
-
-def flags_of(src):
-    return FLAGS if src in KEEPS_PACKED else FLAGS + NO_PACKED
+# then: they are switched off (hipcc's host pass does not know the feature and says so: harmless).
+FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fno-gpu-rdc', '-Wno-unused-value',
+         '-Wno-pass-failed', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def source_hash():
@@ -58,7 +49,7 @@ def _compile(src, hdr_mtime, force):
     spath = os.path.join(CSRC, src)
     if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(spath), hdr_mtime):
         return obj, False
-    subprocess.check_call([HIPCC] + flags_of(src) + ['-c', spath, '-o', obj])
+    subprocess.check_call([HIPCC] + FLAGS + ['-c', spath, '-o', obj])
     return obj, True
 
 
@@ -79,7 +70,7 @@ def _hash_object(force):
 
 def build(force=False, verbose=True):
     os.makedirs(OBJ, exist_ok=True)
-    stamp, line = os.path.join(OBJ, 'flags.txt'), ' '.join([HIPCC] + FLAGS + NO_PACKED + list(KEEPS_PACKED)) + '\n'
+    stamp, line = os.path.join(OBJ, 'flags.txt'), ' '.join([HIPCC] + FLAGS) + '\n'
     if not os.path.exists(stamp) or open(stamp).read() != line:          # objects of other flags are stale
         force = True
     hdr = _deps_mtime()

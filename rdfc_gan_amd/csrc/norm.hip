@@ -192,6 +192,19 @@ __device__ __forceinline__ void load_consts(const float *__restrict__ p, int idx
 constexpr int MAXSEQ = 8;
 struct Moms { float m[MAXSEQ]; };
 
+// s += f^2.  f32 maps: the square is rounded before it is added, in every element, so that the sum does not depend on what the compiler fuses.  Either form
+// is as good, but a statistic's last bit decides which side of zero the next activation's input falls on where that is zero within rounding, and this
+// is the form under which the f32 parity fixtures take upstream's sides.  (The square of a 16-bit value is exact in f32: one form.)
+template <typename T> __device__ __forceinline__ void add_square(float &s, float f) {
+    if constexpr (sizeof(T) == 4) {
+#pragma clang fp contract(off)
+        const float q = f * f;
+        s += q;
+    } else {
+        s = fmaf(f, f, s);
+    }
+}
+
 template <typename T>
 __global__ __launch_bounds__(NT) void stats_kernel(Map m, const T *__restrict__ x, int ld, float *__restrict__ partial) {
     constexpr int VEC = Elem<T>::VEC;
@@ -211,7 +224,7 @@ __global__ __launch_bounds__(NT) void stats_kernel(Map m, const T *__restrict__ 
             for (int v = 0; v < VEC; ++v) {
                 const float f = a.get(v);
                 s[0][v] += f;
-                s[1][v] += f * f;
+                add_square<T>(s[1][v], f);
             }
         };
         row_loop_pf<4>(cx, fetch, add);

@@ -52,3 +52,16 @@ def test_loaded_library_was_built_from_these_sources():
     from rdfc_gan_amd import build, hip
     build.build(verbose=False)
     assert hip.build_hash() == build.source_hash()
+
+
+def test_every_source_is_built_without_packed_f32_instructions(monkeypatch):
+    """hipcc forms packed f32 instructions by itself, some of which have given wrong results on gfx950: no source is compiled with them"""
+    from rdfc_gan_amd import build
+    lines = []
+    monkeypatch.setattr(build.subprocess, 'check_call', lambda cmd, **kw: lines.append(cmd))
+    for src in build._sources():
+        build._compile(src, 0, force=True)
+    assert len(lines) == len(build._sources()) > 10
+    for cmd in lines:
+        assert ' '.join(cmd).count('-Xclang -target-feature -Xclang -packed-fp32-ops') == 1, cmd
+        assert 'v_pk_' not in re.sub(r'//.*', '', open(next(a for a in cmd if a.endswith('.hip'))).read())

@@ -6,6 +6,6 @@ src=$1; out=$2; shift 2
 B=rdfc_gan_amd/csrc/build
 mkdir -p $(dirname $out)
 obj=$(dirname $out)/$(basename $out .so)_$(basename $src .hip).o
-/opt/rocm/bin/hipcc $(python3 -c "from rdfc_gan_amd.build import flags_of; print(*flags_of('$src'))") "$@" -c rdfc_gan_amd/csrc/$src -o $obj || exit 1
+/opt/rocm/bin/hipcc $(python3 -c "from rdfc_gan_amd.build import FLAGS; print(*FLAGS)") "$@" -c rdfc_gan_amd/csrc/$src -o $obj || exit 1
 objs=$(ls $B/*.o | grep -v "/$(basename $src .hip).o")
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $out $objs $obj

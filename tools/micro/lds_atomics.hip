@@ -1,5 +1,5 @@
 // Micro-benchmark: throughput of LDS atomic adds by type (f32 / u32 / u64) and of global f32 atomics, in the access pattern of
-// nlspn.hip's scatter (64 lanes -> 64 consecutive cells, 72 adds per thread).   hipcc --offload-arch=gfx950 -O3 lds_atomics.hip
+// nlspn.hip's scatter (64 lanes -> 64 consecutive cells, 72 adds per thread).   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops lds_atomics.hip
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 constexpr int NT = 256, WN = 1152, ADDS = 72, REP = 8;

@@ -1,5 +1,5 @@
 // Read-only streaming probe (MI355X): which shape of a reduction's read loop reaches the HBM rate the read+write passes get?
-//   hipcc --offload-arch=gfx950 -O3 -o /tmp/read_probe tools/probes/read_probe.hip && /tmp/read_probe
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o /tmp/read_probe tools/probes/read_probe.hip && /tmp/read_probe
 // A 142 MB map (16 x 228 x 304 x 64 f16) is summed per thread; six maps are cycled so every launch reads HBM-cold data.
 #include <hip/hip_runtime.h>
 #include <stdio.h>

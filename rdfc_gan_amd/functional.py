@@ -1131,23 +1131,22 @@ def dropout(x, p, training=True, rng=None):
     return _Dropout.apply(x, threshold, seed, offset, key) if threshold else x
 
 
-def _layout_of(*tensors):
-    """(shape, type, device) of the tensors that a forward pass saves"""
-    return [t if t is None else (t.shape, t.dtype, t.device) for t in tensors]
+# Saved-tensor hooks may return what a forward pass saved with other strides (values moved to the host and back come dense).  The two functions
+# below give it as the kernels read it; another size, type or device is refused.
+def _unpacked_map(t, meta):
+    """a map of (shape, type, device index) -> readable through (pointer, ld)"""
+    if t.shape != meta[0] or t.dtype is not meta[1] or t.get_device() != meta[2]:
+        raise RuntimeError(f'a saved-tensor hook returned {tuple(t.shape)} of {t.dtype} on {t.device} for a map of {tuple(meta[0])} of {meta[1]}')
+    return hip.as_pm(t)
 
 
-def _unpacked(saved, layout, weights=()):
-    """saved tensors as the kernels read them: maps through (pointer, ld), `weights` (positions) as dense rows, the rest dense.  Saved-tensor
-    hooks may return them with other strides than the forward pass had (values moved to the host and back come dense); another shape, type
-    or device is refused."""
-    out = []
-    for i, (t, want) in enumerate(zip(saved, layout)):
-        if t is not None:
-            if (t.shape, t.dtype, t.device) != want:
-                raise RuntimeError(f'a saved-tensor hook returned {tuple(t.shape)} of {t.dtype} on {t.device} for {tuple(want[0])} of {want[1]} on {want[2]}')
-            t = hip.as_pm(t) if t.dim() == 4 else _weight_rows(t, t.dtype) if i in weights else t.contiguous()
-        out.append(t)
-    return out
+def _unpacked_vec(t, numel, dtype, device):
+    """`numel` values of `dtype` -> dense"""
+    if t is None:
+        return None
+    if t.numel() != numel or t.dtype is not dtype or t.get_device() != device:
+        raise RuntimeError(f'a saved-tensor hook returned {t.numel()} values of {t.dtype} on {t.device} for {numel} of {dtype}')
+    return t if t.is_contiguous() else t.contiguous()
 
 
 class _NormResidual(torch.autograd.Function):
@@ -1158,18 +1157,24 @@ class _NormResidual(torch.autograd.Function):
         x = hip.as_pm(x)
         h = hip.as_pm(h) if h is not None else None
         post, pre = (post_w, post_b) if has_post else None, (pre_w, pre_b) if has_pre else None
-        d, y, n, stats = hip.norm_residual(x, h, gate, scale, post, pre, layer, eps, *drop, want_stats=grad_on and any(ctx.needs_input_grad))
-        saved = x, h, gate, scale, post_w, post_b, pre_w, stats, drop[3]
-        ctx.save_for_backward(*saved)
-        ctx.meta = d, has_post, has_pre, _layout_of(*saved)
-        ctx.set_materialize_grads(False)
+        train = grad_on and any(ctx.needs_input_grad)
+        d, y, n, stats = hip.norm_residual(x, h, gate, scale, post, pre, layer, eps, *drop, want_stats=train)
+        if train:
+            ctx.save_for_backward(x, h, gate, scale, post_w, post_b, pre_w, stats, drop[3])
+            ctx.meta = d, has_post, has_pre, (x.shape, x.dtype, x.get_device())
+            ctx.set_materialize_grads(False)
         return y, n
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dn):
-        d, has_post, has_pre, layout = ctx.meta
-        x, h, gate, scale, post_w, post_b, pre_w, stats, key = _unpacked(ctx.saved_tensors, layout)
+        d, has_post, has_pre, meta = ctx.meta
+        x, h, gate, scale, post_w, post_b, pre_w, stats, key = ctx.saved_tensors
+        x, h = _unpacked_map(x, meta), h if h is None else _unpacked_map(h, meta)
+        dev, C = meta[2], d.C
+        gate, stats = _unpacked_vec(gate, d.samples * C, torch.float32, dev), _unpacked_vec(stats, 4 * d.samples * d.rows, torch.float32, dev)
+        scale, post_w, post_b, pre_w = (_unpacked_vec(t, C, torch.float32, dev) for t in (scale, post_w, post_b, pre_w))
+        key = _unpacked_vec(key, 2, torch.int64, dev)
         if dy is None and dn is None:
             return (None,) * 14
         if dy is not None:
@@ -1245,17 +1250,25 @@ class _GatedLinear(torch.autograd.Function):
         x = hip.as_pm(x)
         ctx.dw_dtype = wg.dtype
         wg, wu = (_weight_rows(w, x.dtype) for w in (wg, wu))
-        d, z, pre = hip.gated_linear(x, wg, wu, bg, bu, act, want_pre=grad_on and any(ctx.needs_input_grad))
-        saved = x, wg, wu, bg, bu, pre
-        ctx.save_for_backward(*saved)
-        ctx.meta = d, _layout_of(*saved)
+        train = grad_on and any(ctx.needs_input_grad)
+        d, z, pre = hip.gated_linear(x, wg, wu, bg, bu, act, want_pre=train)
+        if train:
+            ctx.save_for_backward(x, wg, wu, bg, bu, pre)
+            ctx.meta = d, (x.shape, x.dtype, x.get_device())
         return z
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dz):
-        d, layout = ctx.meta
-        x, wg, wu, bg, bu, pre = _unpacked(ctx.saved_tensors, layout, weights=(1, 2))
+        d, meta = ctx.meta
+        x, wg, wu, bg, bu, pre = ctx.saved_tensors
+        x, dev = _unpacked_map(x, meta), meta[2]
+        for w in (wg, wu):
+            if w.shape != (d.F, d.K) or w.dtype is not meta[1] or w.get_device() != dev:
+                raise RuntimeError(f'a saved-tensor hook returned {tuple(w.shape)} of {w.dtype} on {w.device} for weights [{d.F}, {d.K}] of {meta[1]}')
+        wg, wu = _weight_rows(wg, meta[1]), _weight_rows(wu, meta[1])
+        bg, bu = _unpacked_vec(bg, d.F, torch.float32, dev), _unpacked_vec(bu, d.F, torch.float32, dev)
+        pre = _unpacked_vec(pre, d.M * 2 * ((d.F + 31) // 32 * 32), torch.float32, dev)
         need = ctx.needs_input_grad
         dz = hip.as_pm(dz if dz.dtype == x.dtype else dz.to(x.dtype))
         grads = hip.gated_linear_backward(d, x, wg, wu, bg, bu, pre, dz, need[0], ctx.dw_dtype if need[1] or need[2] else None, need[3] or need[4])

@@ -9,6 +9,7 @@ dimension is contiguous and whose pixel stride ``ld = t.stride(2)`` may exceed C
 (a channel slice ``buf[..., a:b]`` of a wider map) -- see include/rdfc_hip.h.
 """
 import ctypes as C
+import functools
 import os
 
 import numpy as np
@@ -1119,7 +1120,10 @@ def norm_residual(x, h, gate, scale, post, pre, layer, eps, threshold, seed, off
     return d, y, n, stats
 
 
-_nr_scratch = {}         # sizes -> floats of scratch
+@functools.lru_cache(maxsize=256)      # (a caller whose sizes never repeat does not fill the memory with them)
+def _nr_scratch(rows, samples, C_, gated):
+    """floats of scratch of a norm_residual backward pass"""
+    return lib().rdfc_norm_residual_scratch_floats(C.byref(NormResidualDesc(rows=rows, samples=samples, C=C_, ldx=C_, ldh=C_)), int(gated))
 
 
 def norm_residual_backward(d, x, h, gate, scale, post, pre, key, stats, dy, dn, want):
@@ -1145,11 +1149,7 @@ def norm_residual_backward(d, x, h, gate, scale, post, pre, key, stats, dy, dn, 
             if w:
                 cols[i] = parts[at] if i else parts[0].view(N, Cc)
                 at += 1
-        key_ = (d.rows, d.samples, Cc, gate is not None)
-        n = _nr_scratch.get(key_)
-        if n is None:
-            n = _nr_scratch[key_] = lib().rdfc_norm_residual_scratch_floats(C.byref(d), int(gate is not None))
-        scratch = torch.empty(n, dtype=torch.float32, device=dev)
+        scratch = torch.empty(_nr_scratch(d.rows, d.samples, Cc, gate is not None), dtype=torch.float32, device=dev)
     _call('rdfc_norm_residual_backward', x, C.byref(d), _a(x), _a(h), _a(gate), _a(scale), _a(pw), _a(pb), _a(qw), _a(key), _a(stats), _a(dy),
           ld(dy) if dy is not None else Cc, _a(dn), ld(dn) if dn is not None else Cc, _a(dx), _a(dh), _a(scratch), *map(_a, cols))
     return (dx, dh, *cols)

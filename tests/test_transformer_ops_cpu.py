@@ -280,6 +280,15 @@ def test_dropout_draws_from_torchs_generator_through_torch(calls, monkeypatch):
     assert all(k.dtype == torch.int64 and k.shape == (2,) for k in keys)
 
 
+def test_scratch_sizes_are_right_and_do_not_pile_up():
+    from rdfc_gan_amd import hip
+    for rows in range(1, 2000):
+        for gated in (False, True):
+            d = hip.NormResidualDesc(rows=rows, samples=2, C=24, ldx=35, ldh=24, dtype=1, layer=1, post=1, pre=1)
+            assert hip._nr_scratch(rows, 2, 24, gated) == hip.lib().rdfc_norm_residual_scratch_floats(ctypes.byref(d), int(gated)) > 0
+    assert hip._nr_scratch.cache_info().currsize <= 256
+
+
 def test_residual_block_with_dropout_has_upstream_indices():
     """use_dropout puts nn.Dropout(0.5) behind the first activation: the second convolution is conv_block.6"""
     from rdfc_gan_amd.generator import ResnetGenerator

@@ -275,6 +275,58 @@ def test_norm_residual_layouts(shape, how, dtype):
     residual_case(shape, dtype, how, True, True, True, True, False, 0.5)
 
 
+def rounded_norm(v, ev, layer, eps):
+    """row norm of v, itself off by ev, in f32 -> (normalised, its error, reciprocal deviation, its relative error), each element's for itself.
+
+    A sum over the channels is a chain of at most 40 additions (eight channels a lane in up to four vectors, then eight halvings): it is off by 40
+    half steps of the sum of absolute terms, the mean by two more.  The root and the division: six."""
+    U, mean = O.U32, lambda t: t.mean(-1, keepdim=True)
+    c, ec = v, ev
+    if layer:
+        c = v - mean(v)
+        ec = ev + mean(ev) + 42 * U * mean(v.abs()) + U * c.abs()
+    var = mean(c * c) + eps
+    r = 1 / var.sqrt()
+    er = 0.5 * (43 * U + 2 * mean(c.abs() * ec) / var) + 6 * U
+    hat = c * r
+    return hat, r * ec + hat.abs() * (er + 2 * U), r, er
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('layer', [False, True], ids=['rms', 'layer'])
+@pytest.mark.parametrize('shape', [(2, 3, 5, 67), (2, 5, 9, 128), (1, 7, 9, 256), (2, 2, 3, 777), (1, 2, 5, 2048)], ids=str)
+def test_norm_residual_small_elements(shape, layer, dtype):
+    """y, n and the gradient of x element by element: bounds that shrink with the element's own terms, not the map's largest value (channels
+    here differ by up to 2^12 in size)"""
+    N, H, W, C = shape
+    U, mean = O.U32, lambda t: t.mean(-1, keepdim=True)
+    size = torch.exp2(-(torch.arange(C) % 13).float())
+    x, h, gy, gn = ((rnd(*shape, seed=30 + i) * size).to(dtype) for i in range(4))
+    gate, scale, pw, qw = rnd(N, C, seed=34, mean=1.0), rnd(C, seed=35), rnd(C, seed=36, std=0.3, mean=1.0), rnd(C, seed=37, std=0.3, mean=1.0)
+    pb, qb = (rnd(C, seed=38) * size, rnd(C, seed=39) * size) if layer else (None, None)
+    v = [t if t is None else t.to(DEV) for t in (x, h, gate, scale, pw, pb, qw, qb, gy, gn)]
+    v[0].requires_grad_(True)
+    y, n = Fh().norm_residual(v[0], v[1], gate=v[2], scale=v[3], post=(v[4], v[5]), pre=(v[6], v[7]), norm='layer' if layer else 'rms', p=0.25, rng=(8, 9))
+    gx, = torch.autograd.grad([y, n], [v[0]], v[8:])
+    x, h, gy, gn, gate, scale, pw, qw = (t.double() for t in (x, h, gy, gn, gate, scale, pw, qw))
+    pb, qb = (torch.zeros(C, dtype=torch.float64) if t is None else t.double() for t in (pb, qb))
+    f = O.dropout(torch.ones(shape), 0.25, 8, 9) * scale * gate[:, None, None, :]
+    hat, e_hat, _, _ = rounded_norm(h, torch.zeros(shape, dtype=torch.float64), layer, 1e-5)
+    want = x + f * (hat * pw + pb)
+    e_y = (f * pw).abs() * e_hat + 8 * U * f.abs() * ((hat * pw).abs() + pb.abs()) + 2 * U * want.abs()
+    check(y, want, e_y, 'y')
+    yhat, e_yhat, r, er = rounded_norm(want, e_y, layer, 1e-5)
+    n64 = yhat * qw + qb
+    check(n, n64, qw.abs() * e_yhat + 2 * U * (n64.abs() + qb.abs()), 'n')
+    g = gn * qw
+    S, Z = mean(g * yhat), mean(g) if layer else torch.zeros_like(mean(g))
+    e_S, e_Z = 43 * U * mean((g * yhat).abs()) + mean(g.abs() * e_yhat), 43 * U * mean(g.abs()) if layer else 0.0
+    inner = g - yhat * S - Z
+    e_inner = yhat.abs() * e_S + S.abs() * e_yhat + e_Z + 6 * U * (g.abs() + (yhat * S).abs() + Z.abs())
+    t = gy + r * inner
+    check(gx, t, r * e_inner + (r * inner).abs() * (er + 2 * U) + 2 * U * (gy.abs() + t.abs()), 'gradient of x')
+
+
 @pytest.mark.parametrize('parts', range(16))
 def test_norm_residual_parts(parts):
     """every combination of post, pre, gate and scale, with and without dropout and either cotangent"""

@@ -2,10 +2,10 @@
 //
 // y[e] = keep(e) ? x[e] * inv : 0.  The backward pass is the same kernel on the cotangent with the same key.
 //
-// HBM bounds it: 16x228x304x64 in bf16 takes 50 us a pass, 284 MB at 5.7 TB/s (a 2 GB copy reaches 4.9 on the same card, and a pass that moved its
+// HBM bounds it: 16x228x304x64 in bf16 takes 50 us a pass, 284 MB at 5.6 TB/s (x + 1 over 2 GB reaches 6.2 on the same card, and a pass that moved its
 // elements one by one took 160).  A generator call is 18 wide multiplications and about 110 other vector instructions for eight elements, by
 // count some 40 us of the same pass on all SIMDs, under the loads: 32 bits an element would take twice that and bind.
-// Small maps are bound by the launch: 8x15x19x512 in f16 2.9 us.
+// Small maps are bound by the launch: 8x15x19x512 in f16 3 us.
 #include "philox.h"
 
 namespace {

@@ -6,9 +6,10 @@
 // elements and the activation and the product happen in registers: g and u never reach memory.
 // Backward, 16-bit maps: the same product again, with dz in the epilogue: dg = dz u act'(g) and du = dz act(g), side by side in one map
 // D [M][2 Fp] (Fp = F rounded up to 32, the columns between zero), with the bias gradients' partial sums in f32 beside the rounding to
-// the map's type.  Keeping g and u instead would round them to 16 bits, and their traffic costs more than the product up to K of about 400
-// (34656 x 256 -> 1024: 142 MB written and 213 read, 70 us at the rate of a copy, against 36 GFLOP).  f32 maps keep them: nothing is rounded, and the
-// product costs fifteen times as much (2280 x 512 -> 1365: 74 us against 14 for an elementwise pass).
+// the map's type (a cotangent beyond f16's range becomes infinite there, as in every block that stores one).  Keeping g and u instead would round
+// them to 16 bits, and at K = 256 their traffic costs about what the product does (34656 x 256 -> 1024: 142 MB written and 213 read, 57 us at the 6.2 TB/s of
+// a large streaming pass, against 62).  f32 maps keep them: nothing is rounded, and the product costs five times as much as an elementwise pass
+// (2280 x 512 -> 1365: 73 us against 14).
 // Then dx = D [Wg; Wu] and [dWg; dWu] = D^T x, the latter split over the pixels and joined in a fixed order.
 #include "common.h"
 
@@ -106,9 +107,10 @@ template <typename T> __global__ __launch_bounds__(NT) void gated_pack_kernel(co
 // 107 registers: three workgroups share a CU, and one's prologue and epilogue run under the others' MFMAs.  That matters more here than a
 // cheaper K loop: at K = 256 half of the forward pass's time is not the K loop (one K-step instead of eight: 33 of 64 us).
 //
-// Measured (16-bit): forward 34656 x 256 -> 1024 60 us, 605 TFLOP/s (a library product of the same size without activation: 73 us);
-// 8816 x 512 -> 2048 52 us (library 79); 34656 x 1024 -> 1024 160 us, 908 TFLOP/s, where the matrix pipes are busy for half of the cycles.  Backward
-// of the first: D 79 (84 with dz read eight bytes a lane in the epilogue), dx 47, dW 45, the joins 6 and 5 us.
+// Measured (16-bit, launches in a row): forward 34656 x 256 -> 1024 62 us, 588 TFLOP/s (a library product of the same size without activation: 72 us);
+// 8816 x 512 -> 2048 with GELU 54 to 56 us (library 76); 34656 x 1024 -> 1024 160 us, 908 TFLOP/s (library 151), where the matrix pipes are busy for
+// half of the cycles.  The first forward + backward: 262 us.  Its launches in a kernel trace, where none overlap (best of 20, the means are up to a sixth
+// longer): forward 65, D 96 (6 % more with dz read eight bytes a lane in the epilogue), dx 58, dW 46, the joins 6 and 5 us.
 // Tried and not kept: fragments read a step ahead in a second register set (no change), steps of 128 bytes in two pairs of slots (two
 // workgroups a CU: 60 -> 70 us at K = 256), eight waves on 256 x 128 with a ring of three 128-byte steps (75 us at K = 256, 174 at K = 1024).
 //

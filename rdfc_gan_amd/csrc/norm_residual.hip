@@ -10,9 +10,9 @@
 // same bytes as reading a saved y) in f32, so neither y nor the dropout mask nor the normalised maps are kept -- four f32 statistics
 // per pixel are.
 //
-// Measured: 8x57x76x1024 f16 (layer norm before the next block) 51 us forward, 284 MB at 5.6 TB/s, and 101 backward, 426 MB at 4.2 TB/s (two waves a
+// Measured: 8x57x76x1024 f16 (layer norm before the next block) 51 us forward, 284 MB at 5.5 TB/s, and 102 backward, 426 MB at 4.2 TB/s (two waves a
 // SIMD: 180 registers, the sums alone are 32; a second row fetched ahead changes nothing), column sums 10.  8x57x76x256 bf16, both norms, gate
-// and dropout: 16 us forward, 31 backward with the column sums.
+// and dropout: 18 us forward, 25 backward and 8 for the column sums.
 //
 // Column sums (gradients of the four norm parameters, of scale and of gate) reduce to four sums per sample and channel:
 //     A = sum D t hhat,  B = sum D t   (t: cotangent of y, D: dropout factor, hhat: normalised h, or h itself without N_post)

@@ -1029,7 +1029,8 @@ class DropoutState:
     """Generator state {seed, counter} in device memory.  Every draw copies it into a key of its own and advances the counter, on the
     current stream: a captured HIP graph draws new masks at every replay, and a backward pass reads its own forward's key.  Without a seed
     one is drawn from torch's CPU generator: states made one after the other draw different masks, and torch.manual_seed repeats
-    them.  Two states of the same seed draw the same masks."""
+    them.  Two states of the same seed draw the same masks.  A forward pass that is run again for its backward pass (activation
+    checkpointing) would draw its next mask from a state: give such a call a pair (seed, offset)."""
 
     def __init__(self, seed=None, device='cuda'):
         seed = int(torch.empty((), dtype=torch.int64, device='cpu').random_()) if seed is None else int(seed)
@@ -1287,7 +1288,7 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act='silu'):
     16-bit map (cast in the call; their gradients are then f32); b_gate, b_up f32 [F], both or neither.  act: 'silu', 'gelu' (exact),
     'sigmoid' or 'relu'.  For the backward pass f32 maps keep both projections (2 F values a pixel); 16-bit
     maps compute them again, and round their cotangents to the map's type before the products with the weights and with x, as every block
-    here stores its cotangents."""
+    here stores its cotangents (so one beyond f16's 65504 becomes infinite, in f32 weight gradients too: a loss scaler sees it)."""
     _check_map(x, 'gated_linear')
     if act not in hip.GATE_ACT:
         raise ValueError(f'act is one of {sorted(hip.GATE_ACT)}, got {act!r}')
